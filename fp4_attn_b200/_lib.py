@@ -58,6 +58,16 @@ SIGNATURES = {
     "nvfp4sim_nvf4_to_f32": ([_P, _P, _P, _L, _P], _I),
     "nvfp4sim_nvf4_to_f16": ([_P, _P, _P, _L, _P], _I),
     "fp4q_quantize": ([_P, _I, _I, _I, _I, _I, _L, _L, _L, _I, _I, _I, _F, _P, _L, _P, _I, _L, _P, _P, _I, _L, _P], _I),
+    "fp4paged_work_size": ([_I, _I], _L),
+    "fp4paged_append": ([_P, _P, _P, _I, _I, _I, _L, _L, _L, _L, _L, _L, _P, _P, _P], _I),
+    "fp4paged_truncate": ([_P, _P, _P, _I, _P], _I),
+    "fp4paged_compact": ([_P, _P, _P, _P, _P, _I, _I, _P], _I),
+    "fp4paged_fork": ([_P, _P, _P, _I, _I, _P], _I),
+    "fp4paged_gather": ([_P, _P, _P, _I, _P, _I, _I, _P], _I),
+    "fp4paged_attention_workspace_size": ([_I, _I, _I, _I], _L),
+    "fp4paged_attention": ([_P, _P, _I, _I, _I, _I, _L, _L, _L, _P, _L, _L, _L, _P, _P, _F, _P, _I, _P, _L, _P], _I),
+    "fp4_sample": ([_P, _I, _I, _I, _L, _P, _P, _P, _P, _P, _P, _P, _P], _I),
+    "fp4_accept_tree": ([_P, _P, _P, _P, _I, _I, _P, _P, _P, _P], _I),
     "fp4q_global_scale": ([_P, _I, _I, _I, _I, _I, _L, _L, _L, _I, _I, _F, _P, _P], _I),
 }
 

@@ -24,7 +24,7 @@ COMMON = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relax
           "-I", CSRC, "-I", os.path.join(ROOT, "include")]
 # Files whose arithmetic must round exactly like the reference: no FMA contraction.
 EXACT = {"quant.cu", "quant_f32.cu", "quant_bf16.cu", "quant_f16.cu", "quant_fused.cu", "nvfp4sim_compat.cu",
-         "qkv_quant.cu"}
+         "qkv_quant.cu", "paged_cache.cu"}
 
 
 def _nvcc() -> str:

@@ -1,0 +1,119 @@
+// paged.cuh -- what the kernels over the paged NVFP4 cache share: the token
+// quantizer and the page lookup.
+//
+// A token is stored by itself (one row per token and KV head, blocks of 16
+// along head_dim, one global scale g per token over all heads), so that it can
+// be moved, shared and dropped without touching its neighbours.
+#pragma once
+
+#include "common.cuh"
+#include "fp4attn.h"
+
+namespace fp4 {
+
+constexpr int PG_D = 128;           // head dim
+constexpr int PG_ROW = PG_D / 2;    // code bytes of a (token, head)
+constexpr int PG_SF = PG_D / 16;    // scale bytes of a (token, head)
+constexpr float PG_TINY = 1.17549435e-38f;  // 2^-126: 1/g of a smaller g overflows
+
+// Device-side error bits of a cache (status[0]); see fp4attn.h.
+enum : int { PG_NO_PAGES = 1, PG_TOO_LONG = 2, PG_BAD_KEEP = 4, PG_SHARED = 8, PG_BAD_SEQ = 16 };
+
+// The slot of row b of a call, -1 where seqs names none.
+__device__ __forceinline__ int pg_seq(const fp4paged_cache& c, const int32_t* seqs, int b) {
+  const int s = seqs ? seqs[b] : b;
+  return s >= 0 && s < c.max_seqs ? s : -1;
+}
+
+// 16 elements at p (16-byte aligned when VEC), as loaded.
+template <int DT, bool VEC>
+struct Block16 {
+  using T = typename In<DT>::T;
+  static constexpr int W = 16 * (int)sizeof(T) / 16;
+  uint4 raw[W];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) reinterpret_cast<T*>(raw)[i] = p[i];
+    }
+  }
+  __device__ __forceinline__ float operator[](int i) const { return In<DT>::f(reinterpret_cast<const T*>(raw)[i]); }
+  __device__ __forceinline__ float absmax() const {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) m = absmax3(m, (*this)[i], (*this)[i + 1]);
+    return m;
+  }
+};
+
+// g of a token from the maximum of its |x|, and 1/g: a subnormal g counts as
+// 0 (1/g would overflow), one that is not finite makes the token NaN.
+__device__ __forceinline__ float pg_global(float m, float& r) {
+  const bool bad = !(m <= 3.402823466e38f);
+  const float g = m < PG_TINY ? 0.0f : m;
+  r = bad || g == 0.0f ? 0.0f : __frcp_rn(g);
+  return bad ? __int_as_float(0x7fc00000) : g;
+}
+
+// A block under 1/g = r (0 in a token of zeros or NaN): eight code bytes and the E4M3 scale byte.
+template <typename Blk>
+__device__ __forceinline__ uint32_t pg_block(const Blk& x, float r, uint2& codes) {
+  float y[16], m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) y[i] = r == 0.0f ? 0.0f : __fmul_rn(x[i], r), m = fmaxf(m, fabsf(y[i]));
+  const uint32_t s8 = e4m3_satfinite(__fmul_rn(m, recip6<FP4_ARITH_F32>()));
+  const float s = e4m3_to_f32((uint8_t)s8), rs = s == 0.0f ? 0.0f : __frcp_rn(s);
+  uint32_t w[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 16; i += 2)  // + 0: a zero's code has no sign
+    w[i >> 3] |= e2m1x2(__fmul_rn(y[i], rs) + 0.0f, __fmul_rn(y[i + 1], rs) + 0.0f) << (4 * (i & 7));
+  codes = make_uint2(w[0], w[1]);
+  return s8;
+}
+
+// A warp quantizes one token of H heads: lane l takes blocks l, l + 32, ...; at(block) is where the block's
+// elements are, put(block, codes, scale) stores it.  Returns the token's g.  Up to NB blocks a lane stay in
+// registers between the maximum and the codes (NB 0: read twice).
+template <int DT, bool VEC, int NB, typename At, typename Put>
+__device__ __forceinline__ float pg_quantize_token(int nblk, At at, Put put) {
+  const int lane = threadIdx.x & 31;
+  float m = 0.0f, r;
+  if constexpr (NB > 0) {
+    Block16<DT, VEC> x[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+      if (lane + 32 * i < nblk) x[i].load(at(lane + 32 * i));
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+      if (lane + 32 * i < nblk) m = nanmax(m, x[i].absmax());
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = nanmax(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float g = pg_global(m, r);
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+      if (lane + 32 * i < nblk) {
+        uint2 c;
+        const uint32_t s = pg_block(x[i], r, c);
+        put(lane + 32 * i, c, s);
+      }
+    return g;
+  } else {
+    Block16<DT, VEC> x;
+    for (int i = lane; i < nblk; i += 32) x.load(at(i)), m = nanmax(m, x.absmax());
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = nanmax(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float g = pg_global(m, r);
+    for (int i = lane; i < nblk; i += 32) {
+      x.load(at(i));
+      uint2 c;
+      const uint32_t s = pg_block(x, r, c);
+      put(i, c, s);
+    }
+    return g;
+  }
+}
+
+}  // namespace fp4

@@ -321,6 +321,120 @@ int fp4attn_decode_ex(const uint8_t* q_codes, const uint8_t* q_scales, const flo
                       const float* v_g, const uint8_t* v_scales16, int len16, int B, int Hq, int Hkv, int D, int len,
                       int Tmax, float scaling, float* out, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Paged NVFP4 KV cache: sequences of different lengths in pages that can be
+ * shared, moved and freed on the device; no reference counterpart (the
+ * reference appends to the HF cache, llama_patch.py:212-215).
+ *
+ * A token is stored by itself, K and V alike: row mode over its H*D channels
+ * (g = max|x|, 0 where that is subnormal; blocks of 16 along head_dim: E4M3
+ * scale s of max|x/g| / 6, E2M1 codes of x/g/s).  A token with a value that is
+ * not finite has g = NaN and zero codes and scales: it stands for NaN.
+ *   codes [num_pages][H][page_size][D/2], scales [num_pages][H][page_size][D/16],
+ *   g [num_pages][page_size];
+ *   page_table [max_seqs][max_pages]: pages of each sequence in order, -1
+ *   past them; lens [max_seqs]; refs [num_pages]: how many sequences hold a
+ *   page, 0 = free.  New pages are the lowest-numbered free ones, in order of
+ *   (row of the call, position).
+ *   status [1]: error bits, or-ed by the calls below: 1 not enough free pages,
+ *   2 a sequence longer than its row of the page table, 4 a keep list that is
+ *   not increasing or leaves its tail, 8 an append or a compaction that would
+ *   write to a shared page (a fork shortened into a page that was full: fork
+ *   it with deep), 16 a sequence index out of range or a fork onto a sequence
+ *   that is not empty.  An append or a fork that would set a bit changes
+ *   nothing else; a compaction leaves that sequence alone.
+ *   work: fp4paged_work_size(num_pages, max_seqs) int32 of scratch.
+ * page_size 16, 32, 64 or 128; D 128; all buffers 16-byte aligned.  seqs [B]
+ * names each row's sequence (distinct; NULL: row b is sequence b).
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  uint8_t* k_codes;
+  uint8_t* k_scales;
+  float* k_g;
+  uint8_t* v_codes;
+  uint8_t* v_scales;
+  float* v_g;
+  int32_t* page_table;
+  int32_t* lens;
+  int32_t* refs;
+  int32_t* status;
+  int32_t* work;
+  int32_t num_pages, page_size, num_kv_heads, head_dim, max_seqs, max_pages;
+} fp4paged_cache;
+
+int64_t fp4paged_work_size(int num_pages, int max_seqs);
+
+/* Quantize and append T new tokens per row, k and v [B,H,T,D] with element
+ * strides (sB, sH, sT) and d contiguous; counts [B]: of row b only the first
+ * counts[b] (NULL: all). */
+int fp4paged_append(const fp4paged_cache* cache, const void* k, const void* v, int in_dtype, int B, int T,
+                    int64_t k_sB, int64_t k_sH, int64_t k_sT, int64_t v_sB, int64_t v_sH, int64_t v_sT,
+                    const int32_t* seqs, const int32_t* counts, void* stream);
+
+/* Row b keeps its first lens[b] tokens (NULL: none) if it has more; pages that
+ * no sequence holds any more become free. */
+int fp4paged_truncate(const fp4paged_cache* cache, const int32_t* lens, const int32_t* seqs, int B, void* stream);
+
+/* Of the last tails[b] tokens of row b (NULL: N) keep those that
+ * keep[b*N .. b*N + counts[b]) lists (increasing, 0 = the tail's first), moved
+ * together; the rest is dropped and its pages freed. */
+int fp4paged_compact(const fp4paged_cache* cache, const int32_t* keep, const int32_t* counts, const int32_t* tails,
+                     const int32_t* seqs, int B, int N, void* stream);
+
+/* Sequences dst[0..n) become copies of src[0..n): full pages are shared, a
+ * last page that is not full is copied; deep != 0: every page is copied.  The
+ * dst sequences are empty before. */
+int fp4paged_fork(const fp4paged_cache* cache, const int32_t* src, const int32_t* dst, int n, int deep, void* stream);
+
+/* Dequantized K and V of the first T tokens, [B,H,T,D] contiguous in
+ * out_dtype, 0 past a sequence's end. */
+int fp4paged_gather(const fp4paged_cache* cache, void* k_out, void* v_out, int out_dtype, const int32_t* seqs, int B,
+                    int T, void* stream);
+
+/* Attention of the last N tokens of each sequence (drafted tokens, already
+ * appended) over the sequence: q [B,Hq,N,D] with element strides and d
+ * contiguous, out [B,N,Hq,D] contiguous in out_dtype.  q is quantized like a
+ * token of the cache (over its Hq*D channels); S = q k^T * scaling, softmax and PV
+ * in higher precision (P is not quantized: its blocks would tie a drafted
+ * token's output to its siblings').  Every token before the last N is visible;
+ * of those, node j is visible to node i where mask[b*m_sB + i*m_sI + j*m_sJ]
+ * is not 0 (NULL: j <= i).  counts [B] (NULL: N): row b has counts[b] <= N
+ * nodes, its last tokens; further rows of out are 0, as is one that sees no
+ * key. */
+int64_t fp4paged_attention_workspace_size(int B, int Hq, int Hkv, int N);
+int fp4paged_attention(const fp4paged_cache* cache, const void* q, int in_dtype, int B, int Hq, int N, int64_t q_sB,
+                       int64_t q_sH, int64_t q_sT, const uint8_t* mask, int64_t m_sB, int64_t m_sI, int64_t m_sJ,
+                       const int32_t* counts, const int32_t* seqs, float scaling, void* out, int out_dtype,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Sampling from given random numbers, one u in [0, 1) per row; logits [R][V]
+ * with row stride ld.  Weights exp((x - max) / temperature[r]) are held as
+ * multiples of 2^-34 of the largest, so every sum is exact and the result does
+ * not depend on an order of summation.  In order of (logit descending, index
+ * ascending) a row keeps the first top_k[r] (<= 0: all), of those the
+ * shortest prefix with a share of at least top_p[r] (>= 1: all), of those
+ * the ones with a weight of at least min_p[r] of the largest; always the
+ * first.  The token is the first kept index i (in index order) whose running
+ * sum exceeds floor(u * sum).  temperature <= 0: the lowest index of the
+ * largest logit.  NaN counts as -inf, +inf as the largest finite value.
+ * logprob[r] (may be NULL) = log softmax(x / temperature)[token], before the
+ * filters (temperature 1 for a greedy row).  A row without a finite logit:
+ * token -1, logprob -inf.  NULL temperature / top_k / top_p / min_p: 1 / 0 / 1 /
+ * 0 for every row.  V <= 262144.
+ * ---------------------------------------------------------------------- */
+int fp4_sample(const void* logits, int in_dtype, int R, int V, int64_t ld, const float* u, const float* temperature,
+               const int32_t* top_k, const float* top_p, const float* min_p, int64_t* tokens, float* logprobs,
+               void* stream);
+
+/* Walk each row's tree from node 0: the lowest child (parents[j] == current,
+ * j > current) whose tokens[j] equals sampled[current] is accepted, until there is
+ * none.  parents, tokens, sampled [B][N], counts [B] (NULL: N) nodes per row.
+ * keep [B][N]: the accepted nodes in order, node 0 first, then N - 1; n [B];
+ * next [B]: sampled at the last accepted node.  A row without nodes: n 0, next -1. */
+int fp4_accept_tree(const int32_t* parents, const int64_t* tokens, const int64_t* sampled, const int32_t* counts,
+                    int B, int N, int32_t* keep, int32_t* n, int64_t* next, void* stream);
+
 /* Measurement aid, no reference counterpart: one CTA per SM (num_ctas <= 0)
  * issues `iters` pairs of back-to-back tcgen05.mma.kind::mxf4nvf4 (M=128,
  * N=128, K=64 each) on fixed pseudo-random NVFP4 operands: the dense NVFP4
