@@ -28,4 +28,5 @@ unsigned int quant_status(bool reset);
 unsigned int decode_status(bool reset);
 unsigned int qkv_status(bool reset);
 unsigned int peak_status(bool reset);
+unsigned int paged_status(bool reset);
 }  // namespace fp4
