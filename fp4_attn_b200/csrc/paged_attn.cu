@@ -246,10 +246,13 @@ __device__ __forceinline__ int owner_of(long long total, long long g, int grid) 
 
 // ------------------------------------------------------------------ attention
 // Warp 0 walks the work list and brings a tile's pages by TMA (a lane per page); warp 1 builds the K scale atoms
-// and issues S^T; warp 2 issues O^T; the softmax warps hold a key per lane and turn S^T into W; the V warps widen
-// V's codes to fp16.  The kernel's code has to stay in the instruction cache (its first form, with the list walked
-// by every role and every loop unrolled, had 130 to 220 KB of it and waited for instructions a third of the time),
-// hence one walker that hands the others what they need through the stage, and loops that stay loops.
+// and issues S^T; warp 2 issues O^T; softmax warps hold a key per lane and 16 rows and turn S^T into W; V warps
+// widen V's codes to fp16.
+//
+// What bounds it is instructions, and first of all fetching them: with the list walked by every role and the rows
+// of a warp unrolled, 110 to 220 KB of code, the instruction caches were 80 % busy.  So one warp walks and hands
+// the others what they need through the stage, every softmax warp has the same 16 rows' worth of code, and what
+// is rare (a moved maximum, masks, an entry's end) stands apart.
 constexpr uint32_t KC = TK * PG_ROW, KS = TK * PG_SF, KG = TK * 4;
 constexpr uint32_t O_VC = KC, O_KS = 2 * KC, O_VS = O_KS + KS, O_KG = O_VS + KS, O_VG = O_KG + KG;
 constexpr uint32_t STAGE = 19 * 1024;  // K codes, V codes, K scales, V scales, K g, V g
@@ -261,25 +264,30 @@ struct TileInfo {
   int b, h, rt, flags;
   int pos, len, base, rows;  // first key, tokens of the sequence, those before the drafted ones, query rows (n * G)
 };
-enum : int { T_FIRST = 1, T_LAST = 2, T_WHOLE = 4, T_SLOT = 8 };  // of the entry, for this CTA; T_SLOT: second partial
+// Of the entry, for this CTA: its first and second tile, its last and the one before, all of its tiles are this
+// CTA's, and which of the CTA's two partials it is.
+enum : int { T_FIRST = 1, T_SECOND = 2, T_LAST = 4, T_PENULT = 8, T_WHOLE = 16, T_SLOT = 32 };
 
 template <int NB, int PL>
 struct Cfg {
-  // softmax warps: four hold 128 keys, eight half of the row chunks each; V warps; 15 in all (128 registers)
-  static constexpr int SW = NB == 16 ? 4 : 8, DW = NB == 16 ? 8 : 4;
-  static constexpr int SW0 = 3, DW0 = SW0 + SW, THREADS = (DW0 + DW) * 32;
-  static constexpr int HALVES = SW / 4, COLS = NB / HALVES, NCH = COLS / 16;  // chunks of 16 rows per softmax warp
+  // Streams: with 16 rows one group of warps would be bound by latency, so two take the tiles in turn, each with
+  // an O, m and l of its own, joined at the entry's end.
+  static constexpr int ST = NB == 16 ? 2 : 1;
+  static constexpr int CHUNKS = NB / 16, GROUPS = CHUNKS * ST;  // groups of four softmax warps, 16 rows each
+  static constexpr int TW = 4 * CHUNKS, VW = 4;                 // softmax and V warps that a tile has
+  static constexpr int SW0 = 3, DW0 = SW0 + 4 * GROUPS, THREADS = (DW0 + VW * ST) * 32;
   static constexpr int NS = 4;
-  static constexpr bool FLUSH = PL == 2;  // O leaves TMEM after every tile (see below)
+  static constexpr bool FLUSH = PL == 2;            // O leaves TMEM after every tile (see below)
+  static constexpr int OB = FLUSH ? 2 * ST : ST;    // O accumulators
   static constexpr uint32_t PBYTES = TK * NB * 2;  // one plane of W
   static constexpr uint32_t OFF_V = NS * STAGE;
   static constexpr uint32_t OFF_P = OFF_V + 2 * V16;
   static constexpr uint32_t OFF_ATOM = OFF_P + 2 * PL * PBYTES;  // K scale atoms, two tiles of 1 KB
   static constexpr uint32_t OFF_Q = OFF_ATOM + 2048;             // query rows, 64-byte swizzle
   static constexpr uint32_t OFF_QSF = OFF_Q + NB * PG_ROW;
-  static constexpr uint32_t SMEM = OFF_QSF + 1024 + 1024;        // + alignment slack
-  static constexpr uint32_t T_S = 0, T_O = 2 * NB, T_SFA = T_O + (FLUSH ? 2 : 1) * NB, T_SFB = T_SFA + 16,
-                            T_END = T_SFB + 8;
+  static constexpr uint32_t OFF_MERGE = OFF_QSF + 1024;  // one stream's O [16][D], c, l on its way to the other
+  static constexpr uint32_t SMEM = OFF_MERGE + (ST == 2 ? 16 * (PG_D + 2) * 4 : 0) + 1024;  // + alignment slack
+  static constexpr uint32_t T_S = 0, T_O = 2 * NB, T_SFA = T_O + OB * NB, T_SFB = T_SFA + 16, T_END = T_SFB + 8;
   static constexpr uint32_t TMEM = T_END <= 128 ? 128 : T_END <= 256 ? 256 : 512;
   static_assert(SMEM <= 227 * 1024 && T_END <= 512 && OFF_QSF % 1024 == 0, "on-chip memory");
 };
@@ -319,7 +327,7 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 
 // mbar_wait of few instructions: bounded by suspended waits of up to 20 us instead of by the clock.
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, unsigned int site) {
-  if (mbar_try_wait(bar, parity)) return true;
+  if (__builtin_expect(mbar_try_wait(bar, parity), 1)) return true;
 #pragma unroll 1
   for (int i = 0; i < 100000; ++i) {
     if (mbar_try_wait_suspend(bar, parity, kSuspendNs)) return true;
@@ -367,6 +375,17 @@ __device__ __forceinline__ void e2m1x8_f16(uint32_t w, uint32_t* o) {
       : "r"(w));
 }
 
+__device__ __forceinline__ float rcp(float x) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float r;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // Sums of 16 values over the lanes: lane l gets that of value l & 15 (half of the values go each step).
 __device__ __forceinline__ float lane_sums16(float (&v)[16]) {
   const int lane = threadIdx.x & 31;
@@ -386,25 +405,26 @@ __global__ void __launch_bounds__(Cfg<NB, PL>::THREADS, 1)
     paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                       const __grid_constant__ AttnArgs a) {
   using C = Cfg<NB, PL>;
-  constexpr int NS = C::NS, SW = C::SW, DW = C::DW, NCH = C::NCH, HALVES = C::HALVES;
+  constexpr int NS = C::NS, ST = C::ST, OB = C::OB;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ __align__(8) uint64_t full[NS], empty[NS], s_full[2], s_free[2], p_full[2], v_full[2], pv_done[2], o_free,
-      qdrain, drained[2];
-  __shared__ __align__(16) float colb[NB], colc[NB], red[4][NB];
+  __shared__ __align__(8) uint64_t full[NS], empty[NS], s_full[2], s_free[2], p_full[2], v_full[2], pv_done[2],
+      o_free[ST], qdrain, drained[2], m_full, m_free;
+  __shared__ __align__(16) float colb[ST][NB], colc[ST][NB], red[C::GROUPS][4][16];
   __shared__ __align__(16) TileInfo info[NS];
   __shared__ int v_first[2];  // the tile of v_full[k] begins a list entry
-  __shared__ volatile int gave_up[2][2];  // [tile & 1][half of the softmax warps]
+  __shared__ volatile int gave_up[2][C::GROUPS];  // [the group's tile & 1][group]
   __shared__ uint32_t tslot;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < NS; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1 + SW + DW);
+    for (int s = 0; s < NS; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1 + C::TW + C::VW);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1), mbar_init(&s_free[i], SW), mbar_init(&drained[i], 1);
-      mbar_init(&p_full[i], SW), mbar_init(&v_full[i], DW), mbar_init(&pv_done[i], 1);
-      gave_up[i][0] = gave_up[i][1] = 0;
+      mbar_init(&s_full[i], 1), mbar_init(&s_free[i], C::TW), mbar_init(&drained[i], 1);
+      mbar_init(&p_full[i], C::TW), mbar_init(&v_full[i], C::VW), mbar_init(&pv_done[i], 1);
+      for (int g = 0; g < C::GROUPS; ++g) gave_up[i][g] = 0;
     }
-    mbar_init(&o_free, SW), mbar_init(&qdrain, 1);
+    for (int i = 0; i < ST; ++i) mbar_init(&o_free[i], C::TW);
+    mbar_init(&qdrain, 1), mbar_init(&m_full, 4), mbar_init(&m_free, 4);
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -438,7 +458,8 @@ __global__ void __launch_bounds__(Cfg<NB, PL>::THREADS, 1)
       const int s = it % NS, h = p.h;
       const TileInfo ti = {
           p.b, h, p.rt,
-          (it == 0 || p.tile == 0 ? T_FIRST : 0) | (p.tile + 1 == p.tiles || it + 1 == n_it ? T_LAST : 0) |
+          (it == 0 || p.tile == 0 ? T_FIRST : it == 1 || p.tile == 1 ? T_SECOND : 0) |
+              (p.tile + 1 == p.tiles || it + 1 == n_it ? T_LAST : p.tile + 2 == p.tiles || it + 2 == n_it ? T_PENULT : 0) |
               (p.tile + 1 == p.tiles && p.tile <= it ? T_WHOLE : 0) | (p.tile < it ? T_SLOT : 0),
           p.tile * TK, p.row.len, p.row.len - p.row.n, p.row.n * a.G};
       int next = -1;
@@ -544,17 +565,20 @@ __global__ void __launch_bounds__(Cfg<NB, PL>::THREADS, 1)
     // ------------------------------------------------------------------ O^T
     if (lane == 0) {
       const uint32_t idesc = idesc_f16_mn(128, NB);
-      int entries = 0;
+      int entries[2] = {0, 0};
 #pragma unroll 1
       for (int it = 0; it < n_it; ++it) {
-        const int k = it & 1;
+        const int k = it & 1, j = it % ST;
         if (!wait_for(&v_full[k], (it >> 1) & 1, 0x605)) break;
         bool first = v_first[k] != 0;
-        if (first && entries++ > 0 && !C::FLUSH && !wait_for(&o_free, (entries - 2) & 1, 0x606)) break;
+        if (first && !C::FLUSH) {
+          const int n = j ? entries[1]++ : entries[0]++;
+          if (n > 0 && !wait_for(&o_free[j], (n - 1) & 1, 0x606)) break;
+        }
         if (!wait_for(&p_full[k], (it >> 1) & 1, 0x607)) break;
         tc_fence_after();
         if (C::FLUSH) first = true;
-        const uint32_t o = tmem + C::T_O + (C::FLUSH ? NB * k : 0);
+        const uint32_t o = tmem + C::T_O + NB * (it % OB);
         const uint64_t vd = MnTile<128>::desc(smem_u32(sm + C::OFF_V) + k * V16);
         const uint64_t wd = MnTile<NB>::desc(smem_u32(sm + C::OFF_P) + k * PL * C::PBYTES);
 #pragma unroll
@@ -570,103 +594,82 @@ __global__ void __launch_bounds__(Cfg<NB, PL>::THREADS, 1)
     }
   } else if (n_it > 0 && warp < C::DW0) {
     // -------------------------------------------------------------- softmax
-    // A half's warps have the row chunks half, half + HALVES, ...; column c of chunk ch is row tile column
-    // (ch * HALVES + half) * 16 + c.  Chunks past the entry's rows are skipped.
-    const int half = (warp - C::SW0) >> 2, quarter = warp & 3;
-    const uint32_t bar_id = 1 + half, lanes = (uint32_t)(quarter * 32) << 16;
-    const int key = quarter * 32 + lane;
-    uint64_t l2[NCH][8];
-    float of[C::FLUSH ? NCH : 1][16];  // O of this lane's channel, when it is kept here
-    auto col_of = [&](int ch) { return (ch * HALVES + half) * 16; };
-    // adds what tile j left in TMEM.  fp32 outputs: the tensor cores cut off what they add to an accumulator, about
-    // 2^-27 of it each time, always towards 0; over a long list that passes what fp32 promises, so O is summed here.
+    const int group = (warp - C::SW0) >> 2, stream = ST == 2 ? group : 0, c0 = ST == 2 ? 0 : group * 16;
+    const int quarter = warp & 3, key = quarter * 32 + lane;
+    const uint32_t bar_id = 1 + group, lanes = (uint32_t)(quarter * 32) << 16;
+    float(&rd)[4][16] = red[group];
+    float *cc = &colc[stream][c0], *cb = &colb[stream][c0];
+    uint64_t l2[8];
+    float of[16];  // O of this lane's channel, when it is summed here
+    // fp32 outputs: the tensor cores cut off what they add to an accumulator, always towards 0 (2e-6 of the result
+    // after 14 tiles), so each tile's product starts anew and O is summed in registers.
     auto flush = [&](int j) {
       const bool ok = warp_wait(&pv_done[j & 1], (j >> 1) & 1, 0x608);
       tc_fence_after();
+      uint32_t o[16];
+      tmem_ld16(tmem + lanes + C::T_O + NB * (j % OB) + c0, o);
+      tmem_ld_wait();
 #pragma unroll
-      for (int ch = 0; ch < NCH; ++ch) {
-        uint32_t o[16];
-        tmem_ld16(tmem + lanes + C::T_O + NB * (j & 1) + col_of(ch), o);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) of[C::FLUSH ? ch : 0][i] += __uint_as_float(o[i]);
-      }
+      for (int i = 0; i < 16; ++i) of[i] += __uint_as_float(o[i]);
       tc_fence_before();
       return ok;
     };
+    int merges = 0;
 #pragma unroll 1
-    for (int it = 0; it < n_it; ++it) {
-      const int s = it % NS, k = it & 1;
+    for (int it = stream; it < n_it; it += ST) {
+      const int s = it % NS, k = it & 1, turn = (it / ST) & 1;
       bool ok = warp_wait(&full[s], (it / NS) & 1, 0x609);
-      const TileInfo ti = info[s];
+      const int flags = info[s].flags, pos0 = info[s].pos, live = info[s].rows - info[s].rt * NB - c0;
+      const int base = info[s].base, len = info[s].len;
+      const int64_t row0 = (((int64_t)info[s].b * a.c.num_kv_heads + info[s].h) * a.RT + info[s].rt) * NB + c0;
+      const int eb = info[s].b, eh = info[s].h, r0 = info[s].rt * NB + c0;
       const uint8_t* st = sm + (size_t)s * STAGE;
       // this key's factors; keys past the end are not visible, whatever the stage holds for them
       float ak = *reinterpret_cast<const float*>(st + O_KG + key * 4);
       float gv = *reinterpret_cast<const float*>(st + O_VG + key * 4);
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[s]);
-      const int pos = ti.pos + key;
-      const bool first = ti.flags & T_FIRST, edge = ti.pos + TK > ti.base;  // drafted tokens, or the sequence's end
-      const int live = ti.rows - ti.rt * NB;  // columns in use
-      if (first) {
+      const int pos = pos0 + key;
+      const bool first = flags & (ST == 2 ? T_FIRST | T_SECOND : T_FIRST);
+      const bool edge = pos0 + TK > base;  // drafted tokens, or the sequence's end
+      const bool idle = C::CHUNKS > 1 && live <= 0;  // no row of the entry in this chunk
+      if (__builtin_expect(first, 0)) {
         // the factors of the rows' scores, and m = -inf
-        if (key < NB / HALVES) {
-          const int c = ((key >> 4) * HALVES + half) * 16 + (key & 15);
-          colb[c] = c < live ? a.q_f[(((int64_t)ti.b * a.c.num_kv_heads + ti.h) * a.RT + ti.rt) * NB + c] : 0.0f;
-          colc[c] = INFINITY;  // W_BIAS - m
+        if (key < 16) {
+          cb[key] = key < live ? a.q_f[row0 + key] : 0.0f;
+          cc[key] = INFINITY;  // W_BIAS - m
         }
 #pragma unroll
-        for (int ch = 0; ch < NCH; ++ch)
+        for (int i = 0; i < 8; ++i) l2[i] = 0ull;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) l2[ch][i] = 0ull;
-        if constexpr (C::FLUSH)
-#pragma unroll
-          for (int ch = 0; ch < NCH; ++ch)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) of[ch][i] = 0.0f;
+        for (int i = 0; i < 16; ++i) of[i] = 0.0f;
         named_bar(bar_id, 128);
       }
-      if (pos >= ti.len) ak = 0.0f, gv = 1.0f;
+      if (pos >= len) ak = 0.0f, gv = 1.0f;
       const float gs = gv >= GV_MIN ? gv : 1.0f;  // 0 and NaN: V^ is 0 there
-      const float lg = gv != gv ? gv : log2f(gs), rg = __frcp_rn(gs) * L_SCALE;
+      const float lg = gv != gv ? gv : lg2(gs), rg = rcp(gs) * L_SCALE;
       ok = warp_wait(&s_full[k], (it >> 1) & 1, 0x60a) && ok;
       tc_fence_after();
-      uint32_t acc[NCH][16];
-#pragma unroll
-      for (int ch = 0; ch < NCH; ++ch)
-        if (ch == 0 || col_of(ch) < live) tmem_ld16(tmem + lanes + C::T_S + NB * k + col_of(ch), acc[ch]);
+      uint32_t acc[16];
+      tmem_ld16(tmem + lanes + C::T_S + NB * k + c0, acc);
       tmem_ld_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&s_free[k]);
-      // x = S scaling log2(e) + log2(g_v), and the largest x - m
-      float x[NCH][16], top = -INFINITY;
-      const uint64_t ak2 = pk2(ak, ak), lg2 = pk2(lg, lg);
-#pragma unroll
-      for (int ch = 0; ch < NCH; ++ch) {
-        if (ch > 0 && col_of(ch) >= live) continue;
-        const int c0 = col_of(ch);
-#pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-          const ulonglong2 b4 = *reinterpret_cast<const ulonglong2*>(&colb[c0 + j]);
-          upk2(fma2(mul2(pk2(__uint_as_float(acc[ch][j]), __uint_as_float(acc[ch][j + 1])), ak2), b4.x, lg2), x[ch][j],
-               x[ch][j + 1]);
-          upk2(fma2(mul2(pk2(__uint_as_float(acc[ch][j + 2]), __uint_as_float(acc[ch][j + 3])), ak2), b4.y, lg2),
-               x[ch][j + 2], x[ch][j + 3]);
-        }
-        if (edge) {
-          // -inf marks what a row does not see
-          const int jn = pos - ti.base, r = ti.rt * NB + c0;
-          uint32_t seen = 0xffffu;
-          if (pos >= ti.len) {
+      if (!idle) {
+        // -inf marks what a row does not see
+        uint32_t seen = 0xffffu;
+        if (__builtin_expect(edge, 0)) {
+          const int jn = pos - base;
+          if (pos >= len) {
             seen = 0u;
           } else if (jn >= 0) {
             if (a.causal) {
-              const int cmin = jn * a.G - r;  // rows of node >= jn
+              const int cmin = jn * a.G - r0;  // rows of node >= jn
               seen = cmin >= 16 ? 0u : cmin <= 0 ? seen : (seen << cmin) & 0xffffu;
             } else {
-              const uint32_t* bits = a.bits + ((int64_t)ti.b * a.N + jn) * a.nw;
-              int i = r / a.G, g = r - i * a.G;
+              const uint32_t* bits = a.bits + ((int64_t)eb * a.N + jn) * a.nw;
+              int i = r0 / a.G, g = r0 - i * a.G;
               seen = 0u;
 #pragma unroll 1
               for (int j = 0; j < 16; ++j) {
@@ -675,105 +678,94 @@ __global__ void __launch_bounds__(Cfg<NB, PL>::THREADS, 1)
               }
             }
           }
-#pragma unroll
-          for (int j = 0; j < 16; ++j) x[ch][j] = (seen >> j) & 1u ? x[ch][j] : -INFINITY;
         }
+        // y = x - m + W_BIAS, x = S scaling log2(e) + log2(g_v)
+        float y[16];
+        auto scores = [&]() {
+          const uint64_t ak2 = pk2(ak, ak), lg2v = pk2(lg, lg);
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-          const float4 c4 = *reinterpret_cast<const float4*>(&colc[c0 + j]);
-          top = max3f(top, x[ch][j] + c4.x, x[ch][j + 1] + c4.y);
-          top = max3f(top, x[ch][j + 2] + c4.z, x[ch][j + 3] + c4.w);
-        }
-      }
-      if (!ok) gave_up[k][half] = 1;
-      bool flushed = false;
-      if (bar_or(bar_id, 128, top > W_BIAS + W_SLACK)) {
-        // some score passed its row's m: every row's m becomes the maximum so far
+          for (int j = 0; j < 16; j += 4) {
+            const ulonglong2 b4 = *reinterpret_cast<const ulonglong2*>(&cb[j]);
+            const ulonglong2 c4 = *reinterpret_cast<const ulonglong2*>(&cc[j]);
+            upk2(fma2(mul2(pk2(__uint_as_float(acc[j]), __uint_as_float(acc[j + 1])), ak2), b4.x, add2(lg2v, c4.x)), y[j],
+                 y[j + 1]);
+            upk2(fma2(mul2(pk2(__uint_as_float(acc[j + 2]), __uint_as_float(acc[j + 3])), ak2), b4.y, add2(lg2v, c4.y)),
+                 y[j + 2], y[j + 3]);
+          }
+          if (__builtin_expect(edge, 0)) {
 #pragma unroll
-        for (int ch = 0; ch < NCH; ++ch) {
-          if (ch > 0 && col_of(ch) >= live) continue;
+            for (int j = 0; j < 16; ++j) y[j] = (seen >> j) & 1u ? y[j] : -INFINITY;
+          }
+        };
+        scores();
+        const float t0 = max3f(max3f(y[0], y[1], y[2]), max3f(y[3], y[4], y[5]), max3f(y[6], y[7], y[8]));
+        const float t1 = max3f(max3f(y[9], y[10], y[11]), max3f(y[12], y[13], y[14]), y[15]);
+        if (!ok) gave_up[turn][group] = 1;
+        bool flushed = false;
+        if (__builtin_expect(bar_or(bar_id, 128, fmaxf(t0, t1) > W_BIAS + W_SLACK), 0)) {
+          // some score passed its row's m: every row's m becomes the maximum so far
           float mx = -INFINITY;
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const float v = redux_max(x[ch][j]);
+            float v = fmaf(__uint_as_float(acc[j]) * ak, cb[j], lg);
+            if (!((seen >> j) & 1u)) v = -INFINITY;
+            v = redux_max(v);
             if (lane == j) mx = v;
           }
-          if (lane < 16) red[quarter][col_of(ch) + lane] = mx;
-        }
-        named_bar(bar_id, 128);
-        float f[NCH], bn[NCH];
-#pragma unroll
-        for (int ch = 0; ch < NCH; ++ch) {
-          const int c = col_of(ch) + (lane & 15);
-          const float old = colc[c];
-          bn[ch] = fminf(old, W_BIAS - fmaxf(fmaxf(red[0][c], red[1][c]), fmaxf(red[2][c], red[3][c])));
-          if (col_of(ch) >= live) bn[ch] = old;
-          f[ch] = bn[ch] == old ? 1.0f : ex2(bn[ch] - old);
-        }
-        named_bar(bar_id, 128);  // colc and red have been read
-        if (quarter == 0 && lane < 16)
-#pragma unroll
-          for (int ch = 0; ch < NCH; ++ch) colc[col_of(ch) + lane] = bn[ch];
-        named_bar(bar_id, 128);
-        if (!first) {
-          // O of the earlier tiles of this list entry, once they are all in
-          if constexpr (C::FLUSH) ok = flush(it - 1) && ok, flushed = true;
-          else ok = warp_wait(&pv_done[(it - 1) & 1], ((it - 1) >> 1) & 1, 0x60b) && ok;
-          tc_fence_after();
-#pragma unroll
-          for (int ch = 0; ch < NCH; ++ch) {
-            if (ch > 0 && col_of(ch) >= live) continue;
+          if (lane < 16) rd[quarter][lane] = mx;
+          named_bar(bar_id, 128);
+          const int c = lane & 15;
+          const float old = cc[c];
+          const float bn = fminf(old, W_BIAS - fmaxf(fmaxf(rd[0][c], rd[1][c]), fmaxf(rd[2][c], rd[3][c])));
+          const float f = bn == old ? 1.0f : ex2(bn - old);
+          named_bar(bar_id, 128);  // cc and rd have been read
+          if (quarter == 0 && lane < 16) cc[c] = bn;
+          named_bar(bar_id, 128);
+          if (!first) {
+            // O of the earlier tiles of this list entry, once they are all in
             uint32_t o[16];
-            if constexpr (!C::FLUSH) {
-              tmem_ld16(tmem + lanes + C::T_O + col_of(ch), o);
+            if constexpr (C::FLUSH) {
+              ok = flush(it - ST) && ok, flushed = true;
+            } else {
+              ok = warp_wait(&pv_done[(it - ST) & 1], ((it - ST) >> 1) & 1, 0x60b) && ok;
+              tc_fence_after();
+              tmem_ld16(tmem + lanes + C::T_O + NB * (it % OB) + c0, o);
               tmem_ld_wait();
             }
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
-              const float f0 = __shfl_sync(0xffffffffu, f[ch], j), f1 = __shfl_sync(0xffffffffu, f[ch], j + 1);
-              l2[ch][j / 2] = mul2(l2[ch][j / 2], pk2(f0, f1));
+              const float f0 = __shfl_sync(0xffffffffu, f, j), f1 = __shfl_sync(0xffffffffu, f, j + 1);
+              l2[j / 2] = mul2(l2[j / 2], pk2(f0, f1));
               if constexpr (C::FLUSH) {
-                of[ch][j] *= f0, of[ch][j + 1] *= f1;
+                of[j] *= f0, of[j + 1] *= f1;
               } else {
                 o[j] = __float_as_uint(__uint_as_float(o[j]) * f0);
                 o[j + 1] = __float_as_uint(__uint_as_float(o[j + 1]) * f1);
               }
             }
-            if constexpr (!C::FLUSH) tmem_st16(tmem + lanes + C::T_O + col_of(ch), o);
+            if constexpr (!C::FLUSH) {
+              tmem_st16(tmem + lanes + C::T_O + NB * (it % OB) + c0, o);
+              tmem_st_wait();
+              tc_fence_before();
+            }
           }
-          if constexpr (!C::FLUSH) tmem_st_wait();
-          tc_fence_before();
+          scores();
         }
-      }
-      if (it >= 2) ok = warp_wait(&pv_done[k], ((it >> 1) - 1) & 1, 0x60c) && ok;  // W's buffer is free
-      uint8_t* wp = sm + C::OFF_P + k * PL * C::PBYTES;
-      const uint64_t rg2 = pk2(rg, rg);
-#pragma unroll
-      for (int ch = 0; ch < NCH; ++ch) {
-        if (ch > 0 && col_of(ch) >= live) continue;
-        const int c0 = col_of(ch);
+        if (it >= 2) ok = warp_wait(&pv_done[k], ((it >> 1) - 1) & 1, 0x60c) && ok;  // W's buffer is free
+        uint8_t* wp = sm + C::OFF_P + k * PL * C::PBYTES;
+        const uint64_t rg2 = pk2(rg, rg);
 #pragma unroll
         for (int j0 = 0; j0 < 16; j0 += 8) {
-          float e[8];
-#pragma unroll
-          for (int j = 0; j < 8; j += 4) {
-            const float4 c4 = *reinterpret_cast<const float4*>(&colc[c0 + j0 + j]);
-            e[j] = ex2(x[ch][j0 + j] + c4.x), e[j + 1] = ex2(x[ch][j0 + j + 1] + c4.y);
-            e[j + 2] = ex2(x[ch][j0 + j + 2] + c4.z), e[j + 3] = ex2(x[ch][j0 + j + 3] + c4.w);
-          }
-          if (edge) {  // (a row that has seen nothing has m = -inf)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) e[j] = x[ch][j0 + j] == -INFINITY ? 0.0f : e[j];
-          }
           uint32_t hi[4], lo[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            l2[ch][j0 / 2 + j] = fma2(pk2(e[2 * j], e[2 * j + 1]), rg2, l2[ch][j0 / 2 + j]);
-            const __half2 h2 = __floats2half2_rn(e[2 * j], e[2 * j + 1]);
+            const float e0 = ex2(y[j0 + 2 * j]), e1 = ex2(y[j0 + 2 * j + 1]);
+            l2[j0 / 2 + j] = fma2(pk2(e0, e1), rg2, l2[j0 / 2 + j]);
+            const __half2 h2 = __floats2half2_rn(e0, e1);
             hi[j] = *reinterpret_cast<const uint32_t*>(&h2);
             if constexpr (PL == 2) {
               const float2 hf = __half22float2(h2);
-              const __half2 r2 = __floats2half2_rn(e[2 * j] - hf.x, e[2 * j + 1] - hf.y);
+              const __half2 r2 = __floats2half2_rn(e0 - hf.x, e1 - hf.y);
               lo[j] = *reinterpret_cast<const uint32_t*>(&r2);
             }
           }
@@ -781,81 +773,101 @@ __global__ void __launch_bounds__(Cfg<NB, PL>::THREADS, 1)
           *reinterpret_cast<uint4*>(wp + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
           if constexpr (PL == 2) *reinterpret_cast<uint4*>(wp + C::PBYTES + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
+        fence_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[k]);
+        if constexpr (C::FLUSH)
+          if (!first && !flushed) ok = flush(it - ST) && ok;
+        // written before this tile's vote, read after it, so the same for all warps of this group
+        if (gave_up[turn][group]) break;
+      } else {
+        if (lane == 0) mbar_arrive(&p_full[k]);
       }
-      fence_async_smem();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[k]);
-      if constexpr (C::FLUSH)
-        if (!first && !flushed) ok = flush(it - 1) && ok;
-      // written before this tile's vote, read after it, so the same for all warps of this half
-      if (gave_up[k][half]) break;
-      if (ti.flags & T_LAST) {
+      if (__builtin_expect(flags & (ST == 2 ? T_LAST | T_PENULT : T_LAST), 0)) {
         // --------------------------------------------- a list entry's end
-        // l of each row: over the lanes here, over the four warps in red
-#pragma unroll
-        for (int ch = 0; ch < NCH; ++ch) {
+        // l of each row: over the lanes here, over the four warps in rd
+        if (!idle) {
           float v[16];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) upk2(l2[ch][j], v[2 * j], v[2 * j + 1]);
+          for (int j = 0; j < 8; ++j) upk2(l2[j], v[2 * j], v[2 * j + 1]);
           const float sum = lane_sums16(v);
-          if (lane < 16) red[quarter][col_of(ch) + lane] = sum;
+          if (lane < 16) rd[quarter][lane] = sum;
+        } else if (lane < 16) {
+          rd[quarter][lane] = 0.0f;
         }
         named_bar(bar_id, 128);
-        const bool whole = ti.flags & T_WHOLE;
-        float* part = a.part + ((int64_t)blockIdx.x * 2 + (ti.flags & T_SLOT ? 1 : 0)) * (NB * (PG_D + 2));
-        if constexpr (C::FLUSH) ok = flush(it) && ok;
-        else ok = warp_wait(&pv_done[k], (it >> 1) & 1, 0x60d) && ok;
-        tc_fence_after();
-        const int all = a.N * a.G - ti.rt * NB;  // columns that the output has
-#pragma unroll
-        for (int ch = 0; ch < NCH; ++ch) {
-          const int c0 = col_of(ch);
-          if (c0 >= all) continue;
+        if constexpr (C::FLUSH) {
+          ok = flush(it) && ok;
+        } else {
+          ok = warp_wait(&pv_done[k], (it >> 1) & 1, 0x60d) && ok;
+          tc_fence_after();
           uint32_t o[16];
-          if constexpr (!C::FLUSH) {
-            tmem_ld16(tmem + lanes + C::T_O + c0, o);
-            tmem_ld_wait();
-          }
-          const int r = ti.rt * NB + c0;
-          int i = r / a.G, g = r - i * a.G;
-          int64_t at = (((int64_t)ti.b * a.N + i) * a.Hq + ti.h * a.G + g) * PG_D + key;  // key: this lane's channel
+          tmem_ld16(tmem + lanes + C::T_O + NB * (it % OB) + c0, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) of[j] = __uint_as_float(o[j]);
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_free[stream]);
+        float* mg = reinterpret_cast<float*>(sm + C::OFF_MERGE);  // [16][D], c [16], l [16]
+        if (ST == 2 && (flags & T_PENULT)) {
+          // the other stream has the last tile and takes this one's share
+          if (merges > 0) warp_wait(&m_free, (merges - 1) & 1, 0x610);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) mg[j * PG_D + key] = of[j];
+          if (key < 16) mg[16 * PG_D + key] = cc[key], mg[16 * PG_D + 16 + key] = (rd[0][key] + rd[1][key]) + (rd[2][key] + rd[3][key]);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&m_full);
+        } else {
+          const bool other = ST == 2 && !(flags & T_FIRST);
+          if (other) warp_wait(&m_full, merges & 1, 0x611);
+          const bool whole = flags & T_WHOLE;
+          float* part = a.part + ((int64_t)blockIdx.x * 2 + (flags & T_SLOT ? 1 : 0)) * (NB * (PG_D + 2));
+          const int all = a.N * a.G - r0;  // columns that the output has
+          int i = r0 / a.G, g = r0 - i * a.G;
+          int64_t at = (((int64_t)eb * a.N + i) * a.Hq + eh * a.G + g) * PG_D + key;  // key: this lane's channel
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const int c = c0 + j;
-            const float l = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
-            const float v = C::FLUSH ? of[C::FLUSH ? ch : 0][j] : __uint_as_float(o[j]);
+            float l = (rd[0][j] + rd[1][j]) + (rd[2][j] + rd[3][j]), v = of[j], c = cc[j];
+            if (other) {
+              const float l1 = mg[16 * PG_D + 16 + j], cj = mg[16 * PG_D + j], cm = fminf(c, cj);
+              const float f0 = c == cm ? 1.0f : ex2(cm - c), f1 = cj == cm ? 1.0f : ex2(cm - cj);
+              v = v * f0 + mg[j * PG_D + key] * f1, l = l * f0 + l1 * f1, c = cm;
+            }
             if (!whole) {
-              part[c * PG_D + key] = v;
-              if (key == 0) part[NB * PG_D + c] = colc[c], part[NB * (PG_D + 1) + c] = l;
-            } else if (c < all) {
-              store_out<DT>(a.out, at, c < live && l != 0.0f ? v * (L_SCALE / l) : 0.0f);
+              part[(c0 + j) * PG_D + key] = v;
+              if (key == 0) part[NB * PG_D + c0 + j] = c, part[NB * (PG_D + 1) + c0 + j] = l;
+            } else if (j < all) {
+              store_out<DT>(a.out, at, j < live && l != 0.0f ? v * (L_SCALE / l) : 0.0f);
             }
             at += PG_D;
             if (++g == a.G) g = 0, at += (int64_t)(a.Hq - a.G) * PG_D;
           }
+          __syncwarp();
+          if (other && lane == 0) mbar_arrive(&m_free);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&o_free);
-        named_bar(bar_id, 128);  // colc and red are free
+        named_bar(bar_id, 128);  // cc and rd are free
       }
+      if (ST == 2 && (flags & (T_FIRST | T_LAST)) == T_LAST) ++merges;
+      else if (ST == 2 && (flags & T_PENULT)) ++merges;
     }
   } else if (n_it > 0) {
     // ---------------------------------------------------------------- V^
-    const int w = warp - C::DW0;
+    const int w = (warp - C::DW0) % C::VW;
 #pragma unroll 1
-    for (int it = 0; it < n_it; ++it) {
+    for (int it = (warp - C::DW0) / C::VW; it < n_it; it += ST) {
       const int s = it % NS, k = it & 1;
       if (!warp_wait(&full[s], (it / NS) & 1, 0x60e)) break;
       const uint8_t* st = sm + (size_t)s * STAGE;
       uint8_t* vb = sm + C::OFF_V + k * V16;
       const int left = info[s].len - info[s].pos, fl = info[s].flags;
       if (it >= 2 && !warp_wait(&pv_done[k], ((it >> 1) - 1) & 1, 0x60f)) break;
-      if (w == 0 && lane == 0) v_first[k] = fl & T_FIRST;
-#pragma unroll
-      for (int i = 0; i < 16 / DW; ++i) {
-        const int key = (i * DW + w) * 8 + (lane & 7), ch = lane >> 3;  // 32 channels from 32 ch
+      if (w == 0 && lane == 0) v_first[k] = fl & (ST == 2 ? T_FIRST | T_SECOND : T_FIRST);
+#pragma unroll 1
+      for (int i = 0; i < 16 / C::VW; ++i) {
+        const int key = (i * C::VW + w) * 8 + (lane & 7), ch = lane >> 3;  // 32 channels from 32 ch
         const uint4 cw = *reinterpret_cast<const uint4*>(st + O_VC + key * 64 + ((ch ^ ((key >> 1) & 3)) << 4));
         uint32_t sc = *reinterpret_cast<const uint16_t*>(st + O_VS + key * 8 + ch * 2);
         const float gv = *reinterpret_cast<const float*>(st + O_VG + key * 4);
