@@ -10,7 +10,7 @@
 // W within fp16 whatever the values' sizes, and leaves code * scale for V^,
 // exact in fp16.  The row sum is l = sum W / g_v, in fp32.
 //
-// The work, tiles of 128 keys of every (sequence, KV head, tile of rows), is
+// The work, tiles of 256 keys of every (sequence, KV head, tile of rows), is
 // one list that the CTAs (one per SM) share out evenly, whatever the lengths;
 // what a CTA did of a list entry that it shares with others goes to the
 // workspace as (m, l, O), and the last kernel joins those in a fixed order.
@@ -32,9 +32,11 @@ FP4_DEFINE_STATUS_READER(paged_status)
 
 namespace {
 
-constexpr int TK = 128;        // keys of a tile
-constexpr float W_BIAS = 12.0f;  // 2^12 of fp16's 2^15 is W at x = m: its smallest step is then 2^-36 of it
-constexpr float W_SLACK = 3.0f;  // m follows once a score passes it by this much, so W <= 2^15
+constexpr int TK = 256, HK = 128;  // keys of a tile, in two halves of 128 (an MMA's rows)
+// W is 2^9 at x = m and at most 2^15: m follows, for all rows at once, when a score passes it by 6.  Half of fp16's
+// smallest step is then 2^-34 of a row's largest W.  (With 2^12 and 3 the maxima of 32 rows of a few thousand keys
+// moved in every second tile, which costs several times a tile without.)
+constexpr float W_BIAS = 9.0f, W_SLACK = 6.0f;
 constexpr float GV_MIN = 7.888609052e-31f;  // 2^-100: V tokens below count as 0, so that 1/g_v sums stay finite
 constexpr float L_SCALE = 0.0009765625f;    // 2^-10, for the same reason
 
@@ -51,7 +53,7 @@ struct AttnArgs {
   const float* q_f;
   const uint32_t* bits;     // [B][N (key)][nw]: which nodes see node j (mask calls)
   const Row* rows;          // [B]
-  const long long* first;   // [B+1] tiles before row b
+  const int* first;         // [B+1] tiles before row b
   float* part;              // [grid][2]: O [NB][D], W_BIAS - m [NB], l [NB]
   int B, Hq, G, N, RT, nw;  // RT: tiles of NB rows that N * G rows take; nw: words of a mask row
   bool causal;
@@ -148,7 +150,7 @@ __global__ void __launch_bounds__(PREP_THREADS) paged_prep_kernel(AttnArgs a, Pr
     }
   } else {
     Row* rows = const_cast<Row*>(a.rows);
-    long long* first = const_cast<long long*>(a.first);
+    int* first = const_cast<int*>(a.first);
     long long sum = 0;
     for (int b0 = 0; b0 < a.B; b0 += PREP_THREADS) {
       const int b = b0 + threadIdx.x;
@@ -178,9 +180,9 @@ __global__ void __launch_bounds__(PREP_THREADS) paged_prep_kernel(AttnArgs a, Pr
         if (w < warp) before += ssum[w];
         sum += ssum[w];
       }
-      if (b < a.B) first[b] = before + v - t;
+      if (b < a.B) first[b] = (int)min(before + v - t, (long long)INT32_MAX);
     }
-    if (threadIdx.x == 0) first[a.B] = sum;
+    if (threadIdx.x == 0) first[a.B] = (int)min(sum, (long long)INT32_MAX);
   }
 }
 
@@ -192,32 +194,38 @@ struct Place {
 };
 
 // Walks the list from tile g0.  The whole warp takes part.
-__device__ __forceinline__ Place place_at(const AttnArgs& a, int NB, long long g0) {
+__device__ __forceinline__ Place place_at(const AttnArgs& a, int NB, int g0) {
   Place p;
-  // the last row whose first tile is not past g0 (rows without tiles share their successor's)
-  int b = 0;
+  // the last row whose first tile is not past g0 (rows without tiles share their successor's); rows come along
+  // with the prefixes, so that the first 32 cost one trip to memory
+  p.b = 0;
+  int before = 0;
 #pragma unroll 1
   for (int b0 = 0; b0 < a.B; b0 += 32) {
     const int k = b0 + (threadIdx.x & 31);
-    const unsigned m = __ballot_sync(0xffffffffu, k < a.B && a.first[k] <= g0);
-    if (m) b = b0 + 31 - __clz(m);
+    const int f = k < a.B ? a.first[k] : INT32_MAX;
+    const int4 r = k < a.B ? *reinterpret_cast<const int4*>(a.rows + k) : make_int4(-1, 0, 0, 0);
+    const unsigned m = __ballot_sync(0xffffffffu, f <= g0);
+    if (m) {
+      const int l = 31 - __clz(m);
+      p.b = b0 + l;
+      before = __shfl_sync(0xffffffffu, f, l);
+      p.row = {__shfl_sync(0xffffffffu, r.x, l), __shfl_sync(0xffffffffu, r.y, l), __shfl_sync(0xffffffffu, r.z, l), 0};
+    }
     if (m != 0xffffffffu) break;
   }
-  p.b = b;
-  p.row = a.rows[b];
-  long long rem = g0 - a.first[b];
-  int per = 0;
+  int rem = g0 - before, per = 0;
 #pragma unroll 1
   for (int rt = 0; rt < a.RT; ++rt) per += tiles_of(p.row, rt, NB, a.G, a.causal);
-  p.h = per ? (int)(rem / per) : 0;
-  rem -= (long long)p.h * per;
+  p.h = per ? rem / per : 0;
+  rem -= p.h * per;
 #pragma unroll 1
   for (p.rt = 0;; ++p.rt) {
     p.tiles = tiles_of(p.row, p.rt, NB, a.G, a.causal);
     if (rem < p.tiles || p.rt + 1 >= a.RT) break;
     rem -= p.tiles;
   }
-  p.tile = (int)rem;
+  p.tile = rem;
   return p;
 }
 
@@ -238,56 +246,59 @@ __device__ __forceinline__ void advance(const AttnArgs& a, int NB, Place& p) {
   } while (p.tiles == 0);
 }
 
-__device__ __forceinline__ long long range_start(long long total, int cta, int grid) { return total * cta / grid; }
-// The CTA whose range holds tile g: the largest with range_start <= g.
-__device__ __forceinline__ int owner_of(long long total, long long g, int grid) {
-  return (int)(((g + 1) * grid - 1) / total);
-}
+// The list's tiles are shared out evenly, the first total % grid CTAs having one more.
+struct Share {
+  int base, more;
+  __device__ __forceinline__ Share(int total, int grid) : base(total / grid), more(total % grid) {}
+  __device__ __forceinline__ int start(int cta) const { return cta * base + min(cta, more); }
+  __device__ __forceinline__ int owner(int g) const {
+    const int big = more * (base + 1);
+    return g < big ? g / (base + 1) : more + (g - big) / base;
+  }
+};
 
 // ------------------------------------------------------------------ attention
 // Warp 0 walks the work list and brings a tile's pages by TMA (a lane per page); warp 1 builds the K scale atoms
-// and issues S^T; warp 2 issues O^T; softmax warps hold a key per lane and 16 rows and turn S^T into W; V warps
-// widen V's codes to fp16.
+// and issues S^T; warp 2 issues O^T; the softmax warps, two keys (one of each half) and 16 rows a lane at a time,
+// turn S^T into W; the V warps widen V's codes to fp16.
 //
-// What bounds it is instructions, and first of all fetching them: with the list walked by every role and the rows
-// of a warp unrolled, 110 to 220 KB of code, the instruction caches were 80 % busy.  So one warp walks and hands
-// the others what they need through the stage, every softmax warp has the same 16 rows' worth of code, and what
-// is rare (a moved maximum, masks, an entry's end) stands apart.
+// What bounds it is instructions.  At first their fetching (with the list walked by every role and all rows of a
+// warp unrolled, 110 to 220 KB of code, the instruction caches were 80 % busy and a third of the stalls), hence
+// one walker that hands on what the others need through the stage, and apart what is rare (a moved maximum, masks,
+// an entry's end).  Then their number: a softmax warp's waits, arrivals and addresses cost about 210 a tile, its
+// 16 rows and 32 keys only 90, hence tiles of 256 keys and as many rows per warp as its registers hold.
 constexpr uint32_t KC = TK * PG_ROW, KS = TK * PG_SF, KG = TK * 4;
 constexpr uint32_t O_VC = KC, O_KS = 2 * KC, O_VS = O_KS + KS, O_KG = O_VS + KS, O_VG = O_KG + KG;
-constexpr uint32_t STAGE = 19 * 1024;  // K codes, V codes, K scales, V scales, K g, V g
-static_assert(O_VG + KG <= STAGE && STAGE % 1024 == 0, "stage");
-constexpr uint32_t V16 = TK * PG_D * 2;  // widened V: two atoms of 64 channels, [128 keys][128 B]
+constexpr uint32_t STAGE = O_VG + KG;  // K codes, V codes, K scales, V scales, K g, V g: 38 KB
+static_assert(STAGE % 1024 == 0, "stage");
+constexpr uint32_t V16 = HK * PG_D * 2;  // widened V of a half: two atoms of 64 channels, [128 keys][128 B]
 
 // A tile of the list, as the producer hands it on.
 struct TileInfo {
   int b, h, rt, flags;
   int pos, len, base, rows;  // first key, tokens of the sequence, those before the drafted ones, query rows (n * G)
 };
-// Of the entry, for this CTA: its first and second tile, its last and the one before, all of its tiles are this
-// CTA's, and which of the CTA's two partials it is.
-enum : int { T_FIRST = 1, T_SECOND = 2, T_LAST = 4, T_PENULT = 8, T_WHOLE = 16, T_SLOT = 32 };
+// Of the entry, for this CTA: its first tile, its last, all of its tiles are this CTA's, and which of the CTA's two
+// partials it is.
+enum : int { T_FIRST = 1, T_LAST = 2, T_WHOLE = 4, T_SLOT = 8 };
 
 template <int NB, int PL>
 struct Cfg {
-  // Streams: with 16 rows one group of warps would be bound by latency, so two take the tiles in turn, each with
-  // an O, m and l of its own, joined at the entry's end.
-  static constexpr int ST = NB == 16 ? 2 : 1;
-  static constexpr int CHUNKS = NB / 16, GROUPS = CHUNKS * ST;  // groups of four softmax warps, 16 rows each
-  static constexpr int TW = 4 * CHUNKS, VW = 4;                 // softmax and V warps that a tile has
-  static constexpr int SW0 = 3, DW0 = SW0 + 4 * GROUPS, THREADS = (DW0 + VW * ST) * 32;
-  static constexpr int NS = 4;
-  static constexpr bool FLUSH = PL == 2;            // O leaves TMEM after every tile (see below)
-  static constexpr int OB = FLUSH ? 2 * ST : ST;    // O accumulators
-  static constexpr uint32_t PBYTES = TK * NB * 2;  // one plane of W
+  static constexpr int GROUPS = NB == 16 ? 1 : 2;         // groups of four softmax warps
+  static constexpr int NCH = NB / 16 / GROUPS;            // chunks of 16 rows that a group has
+  static constexpr int SW = 4 * GROUPS, DW = 12 - SW;     // softmax and V warps; 15 in all, 128 registers
+  static constexpr int SW0 = 3, DW0 = SW0 + SW, THREADS = (DW0 + DW) * 32;
+  static constexpr int NS = NB == 16 ? 3 : 2;
+  static constexpr bool FLUSH = PL == 2;           // O leaves TMEM after every tile (see below)
+  static constexpr int OB = FLUSH ? 2 : 1;         // O accumulators
+  static constexpr uint32_t PBYTES = HK * NB * 2;  // one plane of W of a half
   static constexpr uint32_t OFF_V = NS * STAGE;
-  static constexpr uint32_t OFF_P = OFF_V + 2 * V16;
-  static constexpr uint32_t OFF_ATOM = OFF_P + 2 * PL * PBYTES;  // K scale atoms, two tiles of 1 KB
-  static constexpr uint32_t OFF_Q = OFF_ATOM + 2048;             // query rows, 64-byte swizzle
+  static constexpr uint32_t OFF_P = OFF_V + 2 * V16;             // [tile & 1][half][plane]
+  static constexpr uint32_t OFF_ATOM = OFF_P + 4 * PL * PBYTES;  // K scale atoms, two tiles of 2 KB
+  static constexpr uint32_t OFF_Q = OFF_ATOM + 4096;             // query rows, 64-byte swizzle
   static constexpr uint32_t OFF_QSF = OFF_Q + NB * PG_ROW;
-  static constexpr uint32_t OFF_MERGE = OFF_QSF + 1024;  // one stream's O [16][D], c, l on its way to the other
-  static constexpr uint32_t SMEM = OFF_MERGE + (ST == 2 ? 16 * (PG_D + 2) * 4 : 0) + 1024;  // + alignment slack
-  static constexpr uint32_t T_S = 0, T_O = 2 * NB, T_SFA = T_O + OB * NB, T_SFB = T_SFA + 16, T_END = T_SFB + 8;
+  static constexpr uint32_t SMEM = OFF_QSF + 1024 + 1024;  // + alignment slack
+  static constexpr uint32_t T_S = 0, T_O = 4 * NB, T_SFA = T_O + OB * NB, T_SFB = T_SFA + 32, T_END = T_SFB + 8;
   static constexpr uint32_t TMEM = T_END <= 128 ? 128 : T_END <= 256 ? 256 : 512;
   static_assert(SMEM <= 227 * 1024 && T_END <= 512 && OFF_QSF % 1024 == 0, "on-chip memory");
 };
@@ -307,7 +318,7 @@ struct MnTile {
   static constexpr uint64_t STEP = (16 * ROW) >> 4;
   static __device__ __forceinline__ uint64_t desc(uint32_t base) {
     constexpr SmemLayout lay = NB == 16 ? kSwizzle32B : NB == 32 ? kSwizzle64B : kSwizzle128B;
-    return smem_desc(base, NB == 128 ? TK * 128 : 8 * ROW, 8 * ROW, lay);
+    return smem_desc(base, NB == 128 ? HK * 128 : 8 * ROW, 8 * ROW, lay);
   }
 };
 // kind::f16, fp16 operands, both MN-major (bits 15 and 16), fp32 accumulators.
@@ -323,11 +334,19 @@ __device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t adesc, uint
       : "memory");
 }
 
+// 16 bytes by cp.async, and this thread's arrival at a barrier once its copies are in.
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// mbar_wait of few instructions: bounded by suspended waits of up to 20 us instead of by the clock.
-__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, unsigned int site) {
-  if (__builtin_expect(mbar_try_wait(bar, parity), 1)) return true;
+// mbar_wait of few instructions: bounded by suspended waits of up to 20 us instead of by the clock, and the waiting
+// itself in a function of its own.
+__device__ __noinline__ bool wait_longer(uint64_t* bar, uint32_t parity, unsigned int site) {
 #pragma unroll 1
   for (int i = 0; i < 100000; ++i) {
     if (mbar_try_wait_suspend(bar, parity, kSuspendNs)) return true;
@@ -336,8 +355,18 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, unsigne
   dev_fail(site);
   return false;
 }
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, unsigned int site) {
+  return __builtin_expect(mbar_try_wait(bar, parity), 1) || wait_longer(bar, parity, site);
+}
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned int site) {
   return __all_sync(0xffffffffu, wait_for(bar, parity, site));
+}
+
+// One lane of the warp, in a way the compiler knows.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+  return ok != 0;
 }
 
 __device__ __forceinline__ float redux_max(float v) {
@@ -386,6 +415,41 @@ __device__ __forceinline__ float lg2(float x) {
   return r;
 }
 
+__device__ __forceinline__ void tmem_ld4(uint32_t taddr, uint32_t (&r)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(taddr));
+}
+
+// Which of the rows r0 .. r0 + 15 see keys pos and pos + HK: bits 0-15 and 16-31.  bits: the row's mask words per
+// drafted node (null: node j is seen by node i >= j).
+__device__ __noinline__ uint32_t seen_rows(const uint32_t* bits, int nw, int N, int G, int r0, int pos, int base,
+                                           int len) {
+  uint32_t seen = 0u;
+#pragma unroll 1
+  for (int hf = 0; hf < 2; ++hf, pos += HK) {
+    const int jn = pos - base;
+    uint32_t v = 0xffffu;
+    if (pos >= len) {
+      v = 0u;
+    } else if (jn >= 0 && !bits) {
+      const int cmin = jn * G - r0;  // rows of node >= jn
+      v = cmin >= 16 ? 0u : cmin <= 0 ? v : (v << cmin) & 0xffffu;
+    } else if (jn >= 0) {
+      const uint32_t* w = bits + (int64_t)jn * nw;
+      int i = r0 / G, g = r0 - i * G;
+      v = 0u;
+#pragma unroll 1
+      for (int j = 0; j < 16; ++j) {
+        if (i < N) v |= ((w[i >> 5] >> (i & 31)) & 1u) << j;
+        if (++g == G) g = 0, ++i;
+      }
+    }
+    seen |= v << (16 * hf);
+  }
+  return seen;
+}
+
 // Sums of 16 values over the lanes: lane l gets that of value l & 15 (half of the values go each step).
 __device__ __forceinline__ float lane_sums16(float (&v)[16]) {
   const int lane = threadIdx.x & 31;
@@ -405,26 +469,28 @@ __global__ void __launch_bounds__(Cfg<NB, PL>::THREADS, 1)
     paged_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                       const __grid_constant__ AttnArgs a) {
   using C = Cfg<NB, PL>;
-  constexpr int NS = C::NS, ST = C::ST, OB = C::OB;
+  constexpr int NS = C::NS, NCH = C::NCH;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ __align__(8) uint64_t full[NS], empty[NS], s_full[2], s_free[2], p_full[2], v_full[2], pv_done[2],
-      o_free[ST], qdrain, drained[2], m_full, m_free;
-  __shared__ __align__(16) float colb[ST][NB], colc[ST][NB], red[C::GROUPS][4][16];
+  __shared__ __align__(8) uint64_t full[NS], empty[NS], s_full[2], s_free[2], p_full[2], p_done[2], v_full[2], v_done[2],
+      o_free, qdrain, drained[2];
+  __shared__ __align__(16) float colb[NB], colc[NB], red[NB / 16][4][16];
   __shared__ __align__(16) TileInfo info[NS];
-  __shared__ int v_first[2];  // the tile of v_full[k] begins a list entry
-  __shared__ volatile int gave_up[2][C::GROUPS];  // [the group's tile & 1][group]
+  __shared__ int v_first;                        // the tile of v_full[0] begins a list entry
+  __shared__ volatile int gave_up[2][C::GROUPS];  // [tile & 1][group]
   __shared__ uint32_t tslot;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  // (broadcast: the compiler then knows that a warp's role is one, and keeps what is uniform in it out of the lanes)
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < NS; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1 + C::TW + C::VW);
+    for (int s = 0; s < NS; ++s)
+      mbar_init(&full[s], a.c.page_size < 64 ? 33 : 1), mbar_init(&empty[s], 1 + C::SW + C::DW);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1), mbar_init(&s_free[i], C::TW), mbar_init(&drained[i], 1);
-      mbar_init(&p_full[i], C::TW), mbar_init(&v_full[i], C::VW), mbar_init(&pv_done[i], 1);
+      mbar_init(&s_full[i], 1), mbar_init(&s_free[i], C::SW), mbar_init(&drained[i], 1);
+      mbar_init(&p_full[i], C::SW), mbar_init(&p_done[i], 1);
+      mbar_init(&v_full[i], 4), mbar_init(&v_done[i], 1);
       for (int g = 0; g < C::GROUPS; ++g) gave_up[i][g] = 0;
     }
-    for (int i = 0; i < ST; ++i) mbar_init(&o_free[i], C::TW);
-    mbar_init(&qdrain, 1), mbar_init(&m_full, 4), mbar_init(&m_free, 4);
+    mbar_init(&o_free, C::SW), mbar_init(&qdrain, 1);
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -437,34 +503,36 @@ __global__ void __launch_bounds__(Cfg<NB, PL>::THREADS, 1)
   const uint32_t tmem = tslot;
   pdl_wait();  // the query's codes and the work list
 
-  const long long total = a.first[a.B];
-  const int grid = (int)min((long long)gridDim.x, total);  // CTAs that have tiles
-  const long long g0 = (int)blockIdx.x < grid ? range_start(total, blockIdx.x, grid) : 0;
-  const int n_it = (int)blockIdx.x < grid ? (int)(range_start(total, blockIdx.x + 1, grid) - g0) : 0;
+  const int total = a.first[a.B], grid = min((int)gridDim.x, total);  // CTAs that have tiles
+  int g0 = 0, n_it = 0;
+  if ((int)blockIdx.x < grid) {
+    const Share share(total, grid);
+    g0 = share.start(blockIdx.x), n_it = share.start(blockIdx.x + 1) - g0;
+  }
 
   if (n_it > 0 && warp == 0) {
     // ------------------------------------------------------------- producer
     if (lane == 0) tma_prefetch_desc(&tmK), tma_prefetch_desc(&tmV);
     const int H = a.c.num_kv_heads, P = a.c.page_size, npp = TK / P;  // pages of a tile, a lane each
-    const uint32_t page_bytes = P * 2 * (PG_ROW + PG_SF + 4);
+    // a bulk copy costs about 65 cycles to issue: with small pages the scales and g come by cp.async instead
+    const bool small = P < 64;
+    const uint32_t page_bytes = P * 2 * (PG_ROW + (small ? 0 : PG_SF + 4));
     Place p = place_at(a, NB, g0);
     auto page_of = [&]() -> int {
       const int k = p.tile * npp + lane;  // page of the sequence
       return lane < npp && k * P < p.row.len ? a.c.page_table[(int64_t)p.row.slot * a.c.max_pages + k] : -1;
     };
-    int page = page_of(), issued = 0;
+    int page = page_of(), issued = 0, s = 0, par = 1;
 #pragma unroll 1
     for (int it = 0; it < n_it; ++it) {
-      const int s = it % NS, h = p.h;
-      const TileInfo ti = {
-          p.b, h, p.rt,
-          (it == 0 || p.tile == 0 ? T_FIRST : it == 1 || p.tile == 1 ? T_SECOND : 0) |
-              (p.tile + 1 == p.tiles || it + 1 == n_it ? T_LAST : p.tile + 2 == p.tiles || it + 2 == n_it ? T_PENULT : 0) |
-              (p.tile + 1 == p.tiles && p.tile <= it ? T_WHOLE : 0) | (p.tile < it ? T_SLOT : 0),
-          p.tile * TK, p.row.len, p.row.len - p.row.n, p.row.n * a.G};
+      const int h = p.h;
+      const TileInfo ti = {p.b, h, p.rt,
+                           (it == 0 || p.tile == 0 ? T_FIRST : 0) | (p.tile + 1 == p.tiles || it + 1 == n_it ? T_LAST : 0) |
+                               (p.tile + 1 == p.tiles && p.tile <= it ? T_WHOLE : 0) | (p.tile < it ? T_SLOT : 0),
+                           p.tile * TK, p.row.len, p.row.len - p.row.n, p.row.n * a.G};
       int next = -1;
       if (it + 1 < n_it) advance(a, NB, p), next = page_of();  // in flight while this tile waits for its stage
-      if (it >= NS && !warp_wait(&empty[s], ((it / NS) - 1) & 1, 0x601)) break;
+      if (it >= NS && !warp_wait(&empty[s], par, 0x601)) break;
       const unsigned live = __ballot_sync(0xffffffffu, page >= 0);
       uint8_t* st = sm + (size_t)s * STAGE;
       if (lane == 0) {
@@ -476,13 +544,31 @@ __global__ void __launch_bounds__(Cfg<NB, PL>::THREADS, 1)
         const int64_t row = ((int64_t)page * H + h) * P;
         tma_load_2d(st + lane * P * PG_ROW, &tmK, &full[s], 0, (int)row);
         tma_load_2d(st + O_VC + lane * P * PG_ROW, &tmV, &full[s], 0, (int)row);
-        bulk_load(st + O_KS + lane * P * PG_SF, a.c.k_scales + row * PG_SF, P * PG_SF, &full[s]);
-        bulk_load(st + O_VS + lane * P * PG_SF, a.c.v_scales + row * PG_SF, P * PG_SF, &full[s]);
-        bulk_load(st + O_KG + lane * P * 4, a.c.k_g + (int64_t)page * P, P * 4, &full[s]);
-        bulk_load(st + O_VG + lane * P * 4, a.c.v_g + (int64_t)page * P, P * 4, &full[s]);
+        if (!small) {
+          bulk_load(st + O_KS + lane * P * PG_SF, a.c.k_scales + row * PG_SF, P * PG_SF, &full[s]);
+          bulk_load(st + O_VS + lane * P * PG_SF, a.c.v_scales + row * PG_SF, P * PG_SF, &full[s]);
+          bulk_load(st + O_KG + lane * P * 4, a.c.k_g + (int64_t)page * P, P * 4, &full[s]);
+          bulk_load(st + O_VG + lane * P * 4, a.c.v_g + (int64_t)page * P, P * 4, &full[s]);
+        }
+      }
+      if (small) {
+#pragma unroll 1
+        for (int i = lane; i < TK / 2; i += 32) {  // 16 bytes: the scales of keys 2 i and 2 i + 1
+          const int from = __shfl_sync(0xffffffffu, page, 2 * i / P);
+          const int64_t row = (((int64_t)from * H + h) * P + 2 * i % P) * PG_SF;
+          if (from >= 0) cp_async16(st + O_KS + i * 16, a.c.k_scales + row), cp_async16(st + O_VS + i * 16, a.c.v_scales + row);
+        }
+#pragma unroll 1
+        for (int i = lane; i < TK / 4; i += 32) {  // the g of four keys
+          const int from = __shfl_sync(0xffffffffu, page, 4 * i / P);
+          const int64_t at = (int64_t)from * P + 4 * i % P;
+          if (from >= 0) cp_async16(st + O_KG + i * 16, a.c.k_g + at), cp_async16(st + O_VG + i * 16, a.c.v_g + at);
+        }
+        cp_async_arrive(&full[s]);
       }
       page = next;
       issued = it + 1;
+      if (++s == NS) s = 0, par ^= 1;
     }
     if (lane == 0)
 #pragma unroll 1
@@ -492,13 +578,13 @@ __global__ void __launch_bounds__(Cfg<NB, PL>::THREADS, 1)
     const uint32_t idesc = idesc_nvf4(128, NB);
     uint8_t *qs = sm + C::OFF_Q, *qsf = sm + C::OFF_QSF;
     const uint64_t qdesc = smem_desc(smem_u32(qs), 16, 512, kSwizzle64B);
-    int entries = 0;
+    int entries = 0, s = 0, par = 0;
 #pragma unroll 1
     for (int it = 0; it < n_it; ++it) {
-      const int s = it % NS, k = it & 1;
-      if (!warp_wait(&full[s], (it / NS) & 1, 0x602)) break;
+      const int k = it & 1;
+      if (!warp_wait(&full[s], par, 0x602)) break;
       const uint8_t* st = sm + (size_t)s * STAGE;
-      if (info[s].flags & T_FIRST) {
+      if (__builtin_expect(info[s].flags & T_FIRST, 0)) {
         // a new list entry: its query rows (contiguous; rows past the entry's hold anything, as columns do not mix)
         const int64_t q0 = (((int64_t)info[s].b * a.c.num_kv_heads + info[s].h) * a.RT + info[s].rt) * NB;
         uint4 v[NB / 8];
@@ -526,7 +612,7 @@ __global__ void __launch_bounds__(Cfg<NB, PL>::THREADS, 1)
         }
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) {
+        if (elect_one()) {
           tc_fence_after();
           tmem_cp_sf_atom(tmem + C::T_SFB, smem_desc(smem_u32(qsf), 16, 128, kSwizzleNone));
           tmem_cp_sf_atom(tmem + C::T_SFB + 4, smem_desc(smem_u32(qsf + 512), 16, 128, kSwizzleNone));
@@ -534,28 +620,34 @@ __global__ void __launch_bounds__(Cfg<NB, PL>::THREADS, 1)
         __syncwarp();
       }
       if (it >= 2 && !warp_wait(&s_free[k], ((it >> 1) - 1) & 1, 0x604)) break;
-      uint8_t* at = sm + C::OFF_ATOM + k * 1024;
+      uint8_t* at = sm + C::OFF_ATOM + k * 2048;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 8; ++j) {
         const uint2 sc = *reinterpret_cast<const uint2*>(st + O_KS + (lane + 32 * j) * 8);
-        *reinterpret_cast<uint32_t*>(at + lane * 16 + j * 4) = sc.x;
-        *reinterpret_cast<uint32_t*>(at + 512 + lane * 16 + j * 4) = sc.y;
+        uint8_t* to = at + (j >> 2) * 1024 + lane * 16 + (j & 3) * 4;
+        *reinterpret_cast<uint32_t*>(to) = sc.x;
+        *reinterpret_cast<uint32_t*>(to + 512) = sc.y;
       }
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) {
+      if (elect_one()) {
         tc_fence_after();
-        const uint32_t sfa = tmem + C::T_SFA + 8 * k;
+        const uint32_t sfa = tmem + C::T_SFA + 16 * k, sd = tmem + C::T_S + 2 * NB * k;
         const uint64_t ad = smem_desc(smem_u32(at), 16, 128, kSwizzleNone);
         const uint64_t kd = smem_desc(smem_u32(st), 16, 512, kSwizzle64B);
-        tmem_cp_sf_atom(sfa, ad);
-        tmem_cp_sf_atom(sfa + 4, ad + (512 >> 4));
-        mma_nvf4(tmem + C::T_S + NB * k, kd, qdesc, idesc, sfa, tmem + C::T_SFB, 0u);
-        mma_nvf4(tmem + C::T_S + NB * k, kd + (32 >> 4), qdesc + (32 >> 4), idesc, sfa + 4, tmem + C::T_SFB + 4, 1u);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_cp_sf_atom(sfa + 4 * c, ad + c * (512 >> 4));
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+          for (int kk = 0; kk < 2; ++kk)
+            mma_nvf4(sd + NB * hf, kd + hf * (HK * PG_ROW >> 4) + kk * 2, qdesc + kk * 2, idesc, sfa + 8 * hf + 4 * kk,
+                     tmem + C::T_SFB + 4 * kk, kk);
         tc_commit(&s_full[k]);
         tc_commit(&empty[s]);
       }
       __syncwarp();
+      if (++s == NS) s = 0, par ^= 1;
     }
     if (lane == 0) {
       tc_commit(&drained[0]);  // what was issued completes before TMEM is released
@@ -563,154 +655,179 @@ __global__ void __launch_bounds__(Cfg<NB, PL>::THREADS, 1)
     }
   } else if (n_it > 0 && warp == 2) {
     // ------------------------------------------------------------------ O^T
-    if (lane == 0) {
-      const uint32_t idesc = idesc_f16_mn(128, NB);
-      int entries[2] = {0, 0};
+    const uint32_t idesc = idesc_f16_mn(128, NB);
+    const uint64_t vd0 = MnTile<128>::desc(smem_u32(sm + C::OFF_V)), wd0 = MnTile<NB>::desc(smem_u32(sm + C::OFF_P));
+    int entries = 0;
+    bool ok = true;
 #pragma unroll 1
-      for (int it = 0; it < n_it; ++it) {
-        const int k = it & 1, j = it % ST;
-        if (!wait_for(&v_full[k], (it >> 1) & 1, 0x605)) break;
-        bool first = v_first[k] != 0;
-        if (first && !C::FLUSH) {
-          const int n = j ? entries[1]++ : entries[0]++;
-          if (n > 0 && !wait_for(&o_free[j], (n - 1) & 1, 0x606)) break;
-        }
-        if (!wait_for(&p_full[k], (it >> 1) & 1, 0x607)) break;
+    for (int it = 0; it < n_it && ok; ++it) {
+      const int k = it & 1;
+      if (!warp_wait(&v_full[0], it & 1, 0x605)) break;
+      bool first = v_first != 0;
+      if (first && !C::FLUSH && entries++ > 0 && !warp_wait(&o_free, (entries - 2) & 1, 0x606)) break;
+      if (!warp_wait(&p_full[k], (it >> 1) & 1, 0x607)) break;
+      if (C::FLUSH) first = true;
+      const uint32_t o = tmem + C::T_O + (C::FLUSH ? NB * k : 0);
+#pragma unroll 1
+      for (int hf = 0; hf < 2; ++hf) {
+        if (hf && !(ok = warp_wait(&v_full[1], it & 1, 0x608))) break;
         tc_fence_after();
-        if (C::FLUSH) first = true;
-        const uint32_t o = tmem + C::T_O + NB * (it % OB);
-        const uint64_t vd = MnTile<128>::desc(smem_u32(sm + C::OFF_V) + k * V16);
-        const uint64_t wd = MnTile<NB>::desc(smem_u32(sm + C::OFF_P) + k * PL * C::PBYTES);
+        const uint64_t vd = vd0 + hf * (V16 >> 4), wd = wd0 + (2 * k + hf) * (PL * C::PBYTES >> 4);
+        if (elect_one()) {
 #pragma unroll
-        for (int ks = 0; ks < TK / 16; ++ks)
+          for (int ks = 0; ks < HK / 16; ++ks)
 #pragma unroll
-          for (int pl = 0; pl < PL; ++pl)
-            mma_f16_ss(o, vd + ks * MnTile<128>::STEP, wd + ks * MnTile<NB>::STEP + pl * (C::PBYTES >> 4), idesc,
-                       first && ks == 0 && pl == 0 ? 0u : 1u);
-        tc_commit(&pv_done[k]);
+            for (int pl = 0; pl < PL; ++pl)
+              mma_f16_ss(o, vd + ks * MnTile<128>::STEP, wd + ks * MnTile<NB>::STEP + pl * (C::PBYTES >> 4), idesc,
+                         ks || pl || hf ? 1u : first ? 0u : 1u);
+          tc_commit(&v_done[hf]);
+          if (hf) tc_commit(&p_done[k]);
+        }
+        __syncwarp();
       }
+    }
+    if (lane == 0) {
       tc_commit(&drained[1]);
       mbar_drain(&drained[1], 0);
     }
   } else if (n_it > 0 && warp < C::DW0) {
     // -------------------------------------------------------------- softmax
-    const int group = (warp - C::SW0) >> 2, stream = ST == 2 ? group : 0, c0 = ST == 2 ? 0 : group * 16;
-    const int quarter = warp & 3, key = quarter * 32 + lane;
+    // A group's warps have the chunks of 16 rows group, group + GROUPS, ...; those past the entry's rows are skipped.
+    const int group = (warp - C::SW0) >> 2, quarter = warp & 3, key = quarter * 32 + lane;
     const uint32_t bar_id = 1 + group, lanes = (uint32_t)(quarter * 32) << 16;
-    float(&rd)[4][16] = red[group];
-    float *cc = &colc[stream][c0], *cb = &colb[stream][c0];
-    uint64_t l2[8];
-    float of[16];  // O of this lane's channel, when it is summed here
+    auto col_of = [&](int ch) { return (ch * C::GROUPS + group) * 16; };
+    uint64_t l2[NCH][8];
+    float of[C::FLUSH ? NCH : 1][16];  // O of this lane's channel, when it is summed here
     // fp32 outputs: the tensor cores cut off what they add to an accumulator, always towards 0 (2e-6 of the result
-    // after 14 tiles), so each tile's product starts anew and O is summed in registers.
+    // after 14 tiles of 128), so each tile's product starts anew and O is summed in registers.
     auto flush = [&](int j) {
-      const bool ok = warp_wait(&pv_done[j & 1], (j >> 1) & 1, 0x608);
+      const bool ok = warp_wait(&p_done[j & 1], (j >> 1) & 1, 0x609);
       tc_fence_after();
-      uint32_t o[16];
-      tmem_ld16(tmem + lanes + C::T_O + NB * (j % OB) + c0, o);
-      tmem_ld_wait();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) of[i] += __uint_as_float(o[i]);
+      for (int ch = 0; ch < NCH; ++ch) {
+        uint32_t o[16];
+        tmem_ld16(tmem + lanes + C::T_O + NB * (j & 1) + col_of(ch), o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) of[C::FLUSH ? ch : 0][i] += __uint_as_float(o[i]);
+      }
       tc_fence_before();
       return ok;
     };
-    int merges = 0;
+    int s = 0, par = 0;
 #pragma unroll 1
-    for (int it = stream; it < n_it; it += ST) {
-      const int s = it % NS, k = it & 1, turn = (it / ST) & 1;
-      bool ok = warp_wait(&full[s], (it / NS) & 1, 0x609);
-      const int flags = info[s].flags, pos0 = info[s].pos, live = info[s].rows - info[s].rt * NB - c0;
-      const int base = info[s].base, len = info[s].len;
-      const int64_t row0 = (((int64_t)info[s].b * a.c.num_kv_heads + info[s].h) * a.RT + info[s].rt) * NB + c0;
-      const int eb = info[s].b, eh = info[s].h, r0 = info[s].rt * NB + c0;
+    for (int it = 0; it < n_it; ++it) {
+      const int k = it & 1;
+      bool ok = warp_wait(&full[s], par, 0x60a);
+      const TileInfo ti = info[s];
       const uint8_t* st = sm + (size_t)s * STAGE;
-      // this key's factors; keys past the end are not visible, whatever the stage holds for them
-      float ak = *reinterpret_cast<const float*>(st + O_KG + key * 4);
-      float gv = *reinterpret_cast<const float*>(st + O_VG + key * 4);
+      // the factors of this lane's keys, one of each half; keys past the end are not visible, whatever the stage
+      // holds for them
+      float ak[2], lg[2], rg[2];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        ak[hf] = *reinterpret_cast<const float*>(st + O_KG + (hf * HK + key) * 4);
+        lg[hf] = *reinterpret_cast<const float*>(st + O_VG + (hf * HK + key) * 4);
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[s]);
-      const int pos = pos0 + key;
-      const bool first = flags & (ST == 2 ? T_FIRST | T_SECOND : T_FIRST);
-      const bool edge = pos0 + TK > base;  // drafted tokens, or the sequence's end
-      const bool idle = C::CHUNKS > 1 && live <= 0;  // no row of the entry in this chunk
+      if (++s == NS) s = 0, par ^= 1;
+      const bool first = ti.flags & T_FIRST;
+      const bool edge = ti.pos + TK > ti.base;  // drafted tokens, or the sequence's end
+      const int live = ti.rows - ti.rt * NB;    // columns in use
       if (__builtin_expect(first, 0)) {
         // the factors of the rows' scores, and m = -inf
-        if (key < 16) {
-          cb[key] = key < live ? a.q_f[row0 + key] : 0.0f;
-          cc[key] = INFINITY;  // W_BIAS - m
+        if (key < 16 * NCH) {
+          const int c = col_of(key >> 4) + (key & 15);
+          colb[c] = c < live ? a.q_f[(((int64_t)ti.b * a.c.num_kv_heads + ti.h) * a.RT + ti.rt) * NB + c] : 0.0f;
+          colc[c] = INFINITY;  // W_BIAS - m
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) l2[i] = 0ull;
+        for (int ch = 0; ch < NCH; ++ch)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) of[i] = 0.0f;
+          for (int i = 0; i < 8; ++i) l2[ch][i] = 0ull;
+        if constexpr (C::FLUSH)
+#pragma unroll
+          for (int ch = 0; ch < NCH; ++ch)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) of[ch][i] = 0.0f;
         named_bar(bar_id, 128);
       }
-      if (pos >= len) ak = 0.0f, gv = 1.0f;
-      const float gs = gv >= GV_MIN ? gv : 1.0f;  // 0 and NaN: V^ is 0 there
-      const float lg = gv != gv ? gv : lg2(gs), rg = rcp(gs) * L_SCALE;
-      ok = warp_wait(&s_full[k], (it >> 1) & 1, 0x60a) && ok;
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        if (ti.pos + hf * HK + key >= ti.len) ak[hf] = 0.0f, lg[hf] = 1.0f;
+        const float gs = lg[hf] >= GV_MIN ? lg[hf] : 1.0f;  // 0 and NaN: V^ is 0 there
+        lg[hf] = lg[hf] != lg[hf] ? lg[hf] : lg2(gs), rg[hf] = rcp(gs) * L_SCALE;
+      }
+      ok = warp_wait(&s_full[k], (it >> 1) & 1, 0x60b) && ok;
+      if (it >= 2) ok = warp_wait(&p_done[k], ((it >> 1) - 1) & 1, 0x60c) && ok;  // W's buffer is free
       tc_fence_after();
-      uint32_t acc[16];
-      tmem_ld16(tmem + lanes + C::T_S + NB * k + c0, acc);
-      tmem_ld_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_free[k]);
-      if (!idle) {
-        // -inf marks what a row does not see
-        uint32_t seen = 0xffffu;
+      bool flushed = false;
+#pragma unroll
+      for (int ch = 0; ch < NCH; ++ch) {
+        const int c0 = col_of(ch);
+        if (NB > 16 && c0 >= live) continue;
+        float *cb = colb + c0, *cc = colc + c0;
+        uint32_t seen = 0xffffffffu;  // a bit per row, for each of the two keys
         if (__builtin_expect(edge, 0)) {
-          const int jn = pos - base;
-          if (pos >= len) {
-            seen = 0u;
-          } else if (jn >= 0) {
-            if (a.causal) {
-              const int cmin = jn * a.G - r0;  // rows of node >= jn
-              seen = cmin >= 16 ? 0u : cmin <= 0 ? seen : (seen << cmin) & 0xffffu;
-            } else {
-              const uint32_t* bits = a.bits + ((int64_t)eb * a.N + jn) * a.nw;
-              int i = r0 / a.G, g = r0 - i * a.G;
-              seen = 0u;
-#pragma unroll 1
-              for (int j = 0; j < 16; ++j) {
-                if (i < a.N) seen |= ((bits[i >> 5] >> (i & 31)) & 1u) << j;
-                if (++g == a.G) g = 0, ++i;
-              }
-            }
-          }
+          seen = seen_rows(a.causal ? nullptr : a.bits + (int64_t)ti.b * a.N * a.nw, a.nw, a.N, a.G, ti.rt * NB + c0,
+                           ti.pos + key, ti.base, ti.len);
         }
-        // y = x - m + W_BIAS, x = S scaling log2(e) + log2(g_v)
-        float y[16];
-        auto scores = [&]() {
-          const uint64_t ak2 = pk2(ak, ak), lg2v = pk2(lg, lg);
+        // y = x - m + W_BIAS, x = S scaling log2(e) + log2(g_v); -inf marks what a row does not see
+        float y[2][16];
+#pragma unroll 1
+        for (;;) {
+          uint32_t acc[2][16];
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) tmem_ld16(tmem + lanes + C::T_S + 2 * NB * k + NB * hf + c0, acc[hf]);
+          tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < 16; j += 4) {
             const ulonglong2 b4 = *reinterpret_cast<const ulonglong2*>(&cb[j]);
             const ulonglong2 c4 = *reinterpret_cast<const ulonglong2*>(&cc[j]);
-            upk2(fma2(mul2(pk2(__uint_as_float(acc[j]), __uint_as_float(acc[j + 1])), ak2), b4.x, add2(lg2v, c4.x)), y[j],
-                 y[j + 1]);
-            upk2(fma2(mul2(pk2(__uint_as_float(acc[j + 2]), __uint_as_float(acc[j + 3])), ak2), b4.y, add2(lg2v, c4.y)),
-                 y[j + 2], y[j + 3]);
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+              const uint64_t ak2 = pk2(ak[hf], ak[hf]), lgv = pk2(lg[hf], lg[hf]);
+              upk2(fma2(mul2(pk2(__uint_as_float(acc[hf][j]), __uint_as_float(acc[hf][j + 1])), ak2), b4.x,
+                        add2(lgv, c4.x)),
+                   y[hf][j], y[hf][j + 1]);
+              upk2(fma2(mul2(pk2(__uint_as_float(acc[hf][j + 2]), __uint_as_float(acc[hf][j + 3])), ak2), b4.y,
+                        add2(lgv, c4.y)),
+                   y[hf][j + 2], y[hf][j + 3]);
+            }
           }
           if (__builtin_expect(edge, 0)) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) y[j] = (seen >> j) & 1u ? y[j] : -INFINITY;
+            for (int j = 0; j < 32; ++j) y[j >> 4][j & 15] = (seen >> j) & 1u ? y[j >> 4][j & 15] : -INFINITY;
           }
-        };
-        scores();
-        const float t0 = max3f(max3f(y[0], y[1], y[2]), max3f(y[3], y[4], y[5]), max3f(y[6], y[7], y[8]));
-        const float t1 = max3f(max3f(y[9], y[10], y[11]), max3f(y[12], y[13], y[14]), y[15]);
-        if (!ok) gave_up[turn][group] = 1;
-        bool flushed = false;
-        if (__builtin_expect(bar_or(bar_id, 128, fmaxf(t0, t1) > W_BIAS + W_SLACK), 0)) {
-          // some score passed its row's m: every row's m becomes the maximum so far
-          float mx = -INFINITY;
+          float top = -INFINITY;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            float v = fmaf(__uint_as_float(acc[j]) * ak, cb[j], lg);
-            if (!((seen >> j) & 1u)) v = -INFINITY;
-            v = redux_max(v);
-            if (lane == j) mx = v;
+          for (int j = 0; j < 16; ++j) top = max3f(top, y[0][j], y[1][j]);
+          if (!ok) gave_up[k][group] = 1;
+          // (after the move below no score is above W_BIAS)
+          if (__builtin_expect(!bar_or(bar_id, 128, top > W_BIAS + W_SLACK), 1)) break;
+          // some score passed its row's m: every row's m becomes the maximum so far
+          float(&rd)[4][16] = red[c0 / 16];
+          float mx = -INFINITY;
+          {
+            float v[16];
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+              uint32_t acc[16];
+              tmem_ld16(tmem + lanes + C::T_S + 2 * NB * k + NB * hf + c0, acc);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const float x = fmaf(__uint_as_float(acc[j]) * ak[hf], cb[j], lg[hf]);
+                const float u = (seen >> (16 * hf + j)) & 1u ? x : -INFINITY;
+                v[j] = hf ? fmaxf(v[j], u) : u;
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float u = redux_max(v[j]);
+              if (lane == j) mx = u;
+            }
           }
           if (lane < 16) rd[quarter][lane] = mx;
           named_bar(bar_id, 128);
@@ -725,168 +842,169 @@ __global__ void __launch_bounds__(Cfg<NB, PL>::THREADS, 1)
             // O of the earlier tiles of this list entry, once they are all in
             uint32_t o[16];
             if constexpr (C::FLUSH) {
-              ok = flush(it - ST) && ok, flushed = true;
+              if (!flushed) ok = flush(it - 1) && ok, flushed = true;
             } else {
-              ok = warp_wait(&pv_done[(it - ST) & 1], ((it - ST) >> 1) & 1, 0x60b) && ok;
+              ok = warp_wait(&p_done[(it - 1) & 1], ((it - 1) >> 1) & 1, 0x60d) && ok;
               tc_fence_after();
-              tmem_ld16(tmem + lanes + C::T_O + NB * (it % OB) + c0, o);
+              tmem_ld16(tmem + lanes + C::T_O + c0, o);
               tmem_ld_wait();
             }
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
               const float f0 = __shfl_sync(0xffffffffu, f, j), f1 = __shfl_sync(0xffffffffu, f, j + 1);
-              l2[j / 2] = mul2(l2[j / 2], pk2(f0, f1));
+              l2[ch][j / 2] = mul2(l2[ch][j / 2], pk2(f0, f1));
               if constexpr (C::FLUSH) {
-                of[j] *= f0, of[j + 1] *= f1;
+                of[ch][j] *= f0, of[ch][j + 1] *= f1;
               } else {
                 o[j] = __float_as_uint(__uint_as_float(o[j]) * f0);
                 o[j + 1] = __float_as_uint(__uint_as_float(o[j + 1]) * f1);
               }
             }
             if constexpr (!C::FLUSH) {
-              tmem_st16(tmem + lanes + C::T_O + NB * (it % OB) + c0, o);
+              tmem_st16(tmem + lanes + C::T_O + c0, o);
               tmem_st_wait();
               tc_fence_before();
             }
           }
-          scores();
         }
-        if (it >= 2) ok = warp_wait(&pv_done[k], ((it >> 1) - 1) & 1, 0x60c) && ok;  // W's buffer is free
-        uint8_t* wp = sm + C::OFF_P + k * PL * C::PBYTES;
-        const uint64_t rg2 = pk2(rg, rg);
 #pragma unroll
-        for (int j0 = 0; j0 < 16; j0 += 8) {
-          uint32_t hi[4], lo[4];
+        for (int hf = 0; hf < 2; ++hf) {
+          uint8_t* wp = sm + C::OFF_P + (2 * k + hf) * PL * C::PBYTES;
+          const uint64_t rg2 = pk2(rg[hf], rg[hf]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float e0 = ex2(y[j0 + 2 * j]), e1 = ex2(y[j0 + 2 * j + 1]);
-            l2[j0 / 2 + j] = fma2(pk2(e0, e1), rg2, l2[j0 / 2 + j]);
-            const __half2 h2 = __floats2half2_rn(e0, e1);
-            hi[j] = *reinterpret_cast<const uint32_t*>(&h2);
-            if constexpr (PL == 2) {
-              const float2 hf = __half22float2(h2);
-              const __half2 r2 = __floats2half2_rn(e0 - hf.x, e1 - hf.y);
-              lo[j] = *reinterpret_cast<const uint32_t*>(&r2);
+          for (int j0 = 0; j0 < 16; j0 += 8) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float e0 = ex2(y[hf][j0 + 2 * j]), e1 = ex2(y[hf][j0 + 2 * j + 1]);
+              l2[ch][j0 / 2 + j] = fma2(pk2(e0, e1), rg2, l2[ch][j0 / 2 + j]);
+              const __half2 h2 = __floats2half2_rn(e0, e1);
+              hi[j] = *reinterpret_cast<const uint32_t*>(&h2);
+              if constexpr (PL == 2) {
+                const float2 hf2 = __half22float2(h2);
+                const __half2 r2 = __floats2half2_rn(e0 - hf2.x, e1 - hf2.y);
+                lo[j] = *reinterpret_cast<const uint32_t*>(&r2);
+              }
             }
+            const uint32_t off = mn_chunk<NB>(key, (c0 + j0) / 8);
+            *reinterpret_cast<uint4*>(wp + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if constexpr (PL == 2)
+              *reinterpret_cast<uint4*>(wp + C::PBYTES + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
           }
-          const uint32_t off = mn_chunk<NB>(key, (c0 + j0) / 8);
-          *reinterpret_cast<uint4*>(wp + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          if constexpr (PL == 2) *reinterpret_cast<uint4*>(wp + C::PBYTES + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
-        fence_async_smem();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[k]);
-        if constexpr (C::FLUSH)
-          if (!first && !flushed) ok = flush(it - ST) && ok;
-        // written before this tile's vote, read after it, so the same for all warps of this group
-        if (gave_up[turn][group]) break;
-      } else {
-        if (lane == 0) mbar_arrive(&p_full[k]);
       }
-      if (__builtin_expect(flags & (ST == 2 ? T_LAST | T_PENULT : T_LAST), 0)) {
+      fence_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_free[k]), mbar_arrive(&p_full[k]);
+      if constexpr (C::FLUSH)
+        if (!first && !flushed) ok = flush(it - 1) && ok;
+      // written before a vote of this tile, read after its last, so the same for all warps of this group
+      if (gave_up[k][group]) break;
+      if (__builtin_expect(ti.flags & T_LAST, 0)) {
         // --------------------------------------------- a list entry's end
-        // l of each row: over the lanes here, over the four warps in rd
-        if (!idle) {
+        // l of each row: over the lanes here, over the four warps in red
+#pragma unroll
+        for (int ch = 0; ch < NCH; ++ch) {
           float v[16];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) upk2(l2[j], v[2 * j], v[2 * j + 1]);
+          for (int j = 0; j < 8; ++j) upk2(l2[ch][j], v[2 * j], v[2 * j + 1]);
           const float sum = lane_sums16(v);
-          if (lane < 16) rd[quarter][lane] = sum;
-        } else if (lane < 16) {
-          rd[quarter][lane] = 0.0f;
+          if (lane < 16) red[col_of(ch) / 16][quarter][lane] = sum;
         }
         named_bar(bar_id, 128);
-        if constexpr (C::FLUSH) {
-          ok = flush(it) && ok;
-        } else {
-          ok = warp_wait(&pv_done[k], (it >> 1) & 1, 0x60d) && ok;
-          tc_fence_after();
-          uint32_t o[16];
-          tmem_ld16(tmem + lanes + C::T_O + NB * (it % OB) + c0, o);
-          tmem_ld_wait();
+        const bool whole = ti.flags & T_WHOLE;
+        float* part = a.part + ((int64_t)blockIdx.x * 2 + (ti.flags & T_SLOT ? 1 : 0)) * (NB * (PG_D + 2));
+        if constexpr (C::FLUSH) ok = flush(it) && ok;
+        else ok = warp_wait(&p_done[k], (it >> 1) & 1, 0x60e) && ok;
+        tc_fence_after();
+        if constexpr (C::FLUSH) {  // back to TMEM, to be read column by column
 #pragma unroll
-          for (int j = 0; j < 16; ++j) of[j] = __uint_as_float(o[j]);
-          tc_fence_before();
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&o_free[stream]);
-        float* mg = reinterpret_cast<float*>(sm + C::OFF_MERGE);  // [16][D], c [16], l [16]
-        if (ST == 2 && (flags & T_PENULT)) {
-          // the other stream has the last tile and takes this one's share
-          if (merges > 0) warp_wait(&m_free, (merges - 1) & 1, 0x610);
+          for (int ch = 0; ch < NCH; ++ch) {
+            uint32_t o[16];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) mg[j * PG_D + key] = of[j];
-          if (key < 16) mg[16 * PG_D + key] = cc[key], mg[16 * PG_D + 16 + key] = (rd[0][key] + rd[1][key]) + (rd[2][key] + rd[3][key]);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&m_full);
-        } else {
-          const bool other = ST == 2 && !(flags & T_FIRST);
-          if (other) warp_wait(&m_full, merges & 1, 0x611);
-          const bool whole = flags & T_WHOLE;
-          float* part = a.part + ((int64_t)blockIdx.x * 2 + (flags & T_SLOT ? 1 : 0)) * (NB * (PG_D + 2));
-          const int all = a.N * a.G - r0;  // columns that the output has
-          int i = r0 / a.G, g = r0 - i * a.G;
-          int64_t at = (((int64_t)eb * a.N + i) * a.Hq + eh * a.G + g) * PG_D + key;  // key: this lane's channel
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            float l = (rd[0][j] + rd[1][j]) + (rd[2][j] + rd[3][j]), v = of[j], c = cc[j];
-            if (other) {
-              const float l1 = mg[16 * PG_D + 16 + j], cj = mg[16 * PG_D + j], cm = fminf(c, cj);
-              const float f0 = c == cm ? 1.0f : ex2(cm - c), f1 = cj == cm ? 1.0f : ex2(cm - cj);
-              v = v * f0 + mg[j * PG_D + key] * f1, l = l * f0 + l1 * f1, c = cm;
-            }
-            if (!whole) {
-              part[(c0 + j) * PG_D + key] = v;
-              if (key == 0) part[NB * PG_D + c0 + j] = c, part[NB * (PG_D + 1) + c0 + j] = l;
-            } else if (j < all) {
-              store_out<DT>(a.out, at, j < live && l != 0.0f ? v * (L_SCALE / l) : 0.0f);
-            }
-            at += PG_D;
-            if (++g == a.G) g = 0, at += (int64_t)(a.Hq - a.G) * PG_D;
+            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(of[ch][j]);
+            tmem_st16(tmem + lanes + C::T_O + NB * k + col_of(ch), o);
           }
-          __syncwarp();
-          if (other && lane == 0) mbar_arrive(&m_free);
+          tmem_st_wait();
         }
-        named_bar(bar_id, 128);  // cc and rd are free
+        const int all = min(NB, a.N * a.G - ti.rt * NB);  // columns that the output has
+#pragma unroll 1
+        for (int ch = 0; ch < NCH; ++ch) {
+          const int c0 = col_of(ch), r0 = ti.rt * NB + c0;
+          if (c0 >= all) break;
+          float(&rd)[4][16] = red[c0 / 16];
+          // lane j (and j + 16): what row j needs
+          const float l = (rd[0][lane & 15] + rd[1][lane & 15]) + (rd[2][lane & 15] + rd[3][lane & 15]);
+          const float scale = c0 + (lane & 15) < live && l != 0.0f ? L_SCALE / l : 0.0f;
+          if (!whole && key < 16) part[NB * PG_D + c0 + key] = colc[c0 + key], part[NB * (PG_D + 1) + c0 + key] = l;
+          int i = r0 / a.G, g = r0 - i * a.G;
+          int64_t at = (((int64_t)ti.b * a.N + i) * a.Hq + ti.h * a.G + g) * PG_D + key;  // key: this lane's channel
+          const uint32_t to = tmem + lanes + C::T_O + (C::FLUSH ? NB * k : 0) + c0;
+          float* pp = part + c0 * PG_D + key;
+#pragma unroll 1
+          for (int j0 = 0; j0 < 16; j0 += 4) {
+            uint32_t o[4];
+            tmem_ld4(to + j0, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 4; ++j, pp += PG_D) {
+              const float v = __uint_as_float(o[j]), f = __shfl_sync(0xffffffffu, scale, j0 + j);
+              if (!whole) *pp = v;
+              else if (c0 + j0 + j < all) store_out<DT>(a.out, at, f == 0.0f ? 0.0f : v * f);
+              at += PG_D;
+              if (++g == a.G) g = 0, at += (int64_t)(a.Hq - a.G) * PG_D;
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_free);
+        named_bar(bar_id, 128);  // colc and red are free
       }
-      if (ST == 2 && (flags & (T_FIRST | T_LAST)) == T_LAST) ++merges;
-      else if (ST == 2 && (flags & T_PENULT)) ++merges;
     }
   } else if (n_it > 0) {
     // ---------------------------------------------------------------- V^
-    const int w = (warp - C::DW0) % C::VW;
+    // four warps per half: both halves at once with eight, in turn with four
+    const int w = (warp - C::DW0) & 3;
+    int s = 0, par = 0;
+    bool ok = true;
 #pragma unroll 1
-    for (int it = (warp - C::DW0) / C::VW; it < n_it; it += ST) {
-      const int s = it % NS, k = it & 1;
-      if (!warp_wait(&full[s], (it / NS) & 1, 0x60e)) break;
+    for (int it = 0; it < n_it && ok; ++it) {
+      ok = warp_wait(&full[s], par, 0x60f);
+      if (!ok) break;
       const uint8_t* st = sm + (size_t)s * STAGE;
-      uint8_t* vb = sm + C::OFF_V + k * V16;
       const int left = info[s].len - info[s].pos, fl = info[s].flags;
-      if (it >= 2 && !warp_wait(&pv_done[k], ((it >> 1) - 1) & 1, 0x60f)) break;
-      if (w == 0 && lane == 0) v_first[k] = fl & (ST == 2 ? T_FIRST | T_SECOND : T_FIRST);
 #pragma unroll 1
-      for (int i = 0; i < 16 / C::VW; ++i) {
-        const int key = (i * C::VW + w) * 8 + (lane & 7), ch = lane >> 3;  // 32 channels from 32 ch
-        const uint4 cw = *reinterpret_cast<const uint4*>(st + O_VC + key * 64 + ((ch ^ ((key >> 1) & 3)) << 4));
-        uint32_t sc = *reinterpret_cast<const uint16_t*>(st + O_VS + key * 8 + ch * 2);
-        const float gv = *reinterpret_cast<const float*>(st + O_VG + key * 4);
-        // tokens past the end, NaN tokens and those below GV_MIN contribute nothing (NaN comes in through W)
-        if (!(gv >= GV_MIN) || key >= left) sc = 0u;
-        const uint32_t s2 = e4m3x2_f16x2(sc), s0 = __byte_perm(s2, s2, 0x1010), s1 = __byte_perm(s2, s2, 0x3232);
-        uint32_t o[16];
-        e2m1x8_f16(cw.x, o), e2m1x8_f16(cw.y, o + 4), e2m1x8_f16(cw.z, o + 8), e2m1x8_f16(cw.w, o + 12);
+      for (int hf = (warp - C::DW0) >> 2; hf < 2; hf += C::DW / 4) {
+        if (it >= 1 && !(ok = warp_wait(&v_done[hf], (it - 1) & 1, 0x610))) break;
+        if (hf == 0 && w == 0 && lane == 0) v_first = fl & T_FIRST;
+        uint8_t* vb = sm + C::OFF_V + hf * V16;
+#pragma unroll 2
+        for (int i = 0; i < 4; ++i) {
+          const int r = (i * 4 + w) * 8 + (lane & 7), key = hf * HK + r, ch = lane >> 3;  // 32 channels from 32 ch
+          const uint4 cw = *reinterpret_cast<const uint4*>(st + O_VC + key * 64 + ((ch ^ ((r >> 1) & 3)) << 4));
+          uint32_t sc = *reinterpret_cast<const uint16_t*>(st + O_VS + key * 8 + ch * 2);
+          const float gv = *reinterpret_cast<const float*>(st + O_VG + key * 4);
+          // tokens past the end, NaN tokens and those below GV_MIN contribute nothing (NaN comes in through W)
+          if (!(gv >= GV_MIN) || key >= left) sc = 0u;
+          const uint32_t s2 = e4m3x2_f16x2(sc), s0 = __byte_perm(s2, s2, 0x1010), s1 = __byte_perm(s2, s2, 0x3232);
+          uint32_t o[16];
+          e2m1x8_f16(cw.x, o), e2m1x8_f16(cw.y, o + 4), e2m1x8_f16(cw.z, o + 8), e2m1x8_f16(cw.w, o + 12);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) o[j] = hmul2_u32(o[j], j < 8 ? s0 : s1);
-        const uint32_t row = (ch >> 1) * (TK * 128) + key * 128;
+          for (int j = 0; j < 16; ++j) o[j] = hmul2_u32(o[j], j < 8 ? s0 : s1);
+          const uint32_t row = (ch >> 1) * (HK * 128) + r * 128;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<uint4*>(vb + row + ((((ch & 1) * 4 + j) ^ (key & 7)) << 4)) =
-              make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<uint4*>(vb + row + ((((ch & 1) * 4 + j) ^ (r & 7)) << 4)) =
+                make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_full[hf]);
       }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[s]), mbar_arrive(&v_full[k]);
+      if (lane == 0) mbar_arrive(&empty[s]);
+      if (++s == NS) s = 0, par ^= 1;
     }
   }
   pdl_launch();
@@ -910,7 +1028,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(AttnArgs a, int grid_ma
   if (r >= a.N * a.G) return;
   const Row row = a.rows[b];
   const int tiles = tiles_of(row, rt, NB, a.G, a.causal);
-  const long long total = a.first[a.B];
+  const int total = a.first[a.B];
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (tiles > 0) {
     int per = 0, before = 0;
@@ -919,15 +1037,15 @@ __global__ void __launch_bounds__(256) paged_join_kernel(AttnArgs a, int grid_ma
       if (i < rt) before += t;
       per += t;
     }
-    const long long t0 = a.first[b] + (long long)h * per + before, t1 = t0 + tiles - 1;
-    const int grid = (int)min((long long)grid_max, total);
-    const int c0 = owner_of(total, t0, grid), c1 = owner_of(total, t1, grid);
+    const int t0 = a.first[b] + h * per + before, t1 = t0 + tiles - 1;
+    const Share share(total, min(grid_max, total));
+    const int c0 = share.owner(t0), c1 = share.owner(t1);
     if (c0 == c1) return;
     if (r < row.n * a.G) {
       // CTA c0's share is its first segment if its range starts with this entry, else its last; the others' is
       // their first
       auto slot = [&](int i) {
-        return a.part + ((int64_t)i * 2 + (i == c0 && range_start(total, c0, grid) < t0 ? 1 : 0)) * (NB * (PG_D + 2));
+        return a.part + ((int64_t)i * 2 + (i == c0 && share.start(c0) < t0 ? 1 : 0)) * (NB * (PG_D + 2));
       };
       float m = INFINITY;  // W_BIAS - the largest m
       for (int i = c0 + lane; i <= c1; i += 32) m = fminf(m, slot(i)[NB * PG_D + c]);
@@ -996,7 +1114,7 @@ Layout layout_of(int B, int Hq, int Hkv, int N, bool fp32) {
   L.bits = L.g + piece(qrows * 4);
   L.rows = L.bits + piece(tok * L.nw * 4);
   L.first = L.rows + piece((int64_t)B * sizeof(Row));
-  L.part = L.first + piece((int64_t)(B + 1) * 8);
+  L.part = L.first + piece((int64_t)(B + 1) * 4);
   L.bytes = L.part + piece((int64_t)L.grid * 2 * L.NB * (PG_D + 2) * 4);
   return L;
 }
@@ -1076,6 +1194,9 @@ extern "C" int fp4paged_attention(const fp4paged_cache* cache, const void* q, in
   if (B > 65535 || (int64_t)H * L.RT > 65535 || (int64_t)N * (Hq / H) > INT32_MAX / 2 ||
       (int64_t)B * N > INT32_MAX / 2)
     return set_error(FP4ATTN_ERR_UNSUPPORTED, "more than 65535 rows or (KV head, row tile) pairs");
+  // the work list is counted in 32 bits
+  const int64_t most = ((int64_t)cache->max_pages * cache->page_size + TK - 1) / TK * L.RT * H * B;
+  if (most > INT32_MAX) return set_error(FP4ATTN_ERR_UNSUPPORTED, "2^31 or more key tiles");
   const int64_t krows = (int64_t)cache->num_pages * H * cache->page_size;
   if (krows > INT32_MAX) return set_error(FP4ATTN_ERR_UNSUPPORTED, "the cache has 2^31 or more (token, head) rows");
   uint8_t* w = static_cast<uint8_t*>(workspace);
@@ -1083,7 +1204,7 @@ extern "C" int fp4paged_attention(const fp4paged_cache* cache, const void* q, in
   a.c = *cache;
   a.q_codes = w, a.q_scales = w + L.scales, a.q_f = reinterpret_cast<float*>(w + L.g);
   a.bits = reinterpret_cast<uint32_t*>(w + L.bits), a.rows = reinterpret_cast<Row*>(w + L.rows);
-  a.first = reinterpret_cast<long long*>(w + L.first), a.part = reinterpret_cast<float*>(w + L.part);
+  a.first = reinterpret_cast<int*>(w + L.first), a.part = reinterpret_cast<float*>(w + L.part);
   a.B = B, a.Hq = Hq, a.G = Hq / H, a.N = N, a.RT = L.RT, a.nw = L.nw;
   a.causal = mask == nullptr, a.scaling = scaling, a.out = out;
   const PrepArgs p{q, q_sB, q_sH, q_sT, mask, m_sB, m_sI, m_sJ, counts, seqs, L.NB,
