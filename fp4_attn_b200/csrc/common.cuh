@@ -112,16 +112,19 @@ template <>
 struct In<FP4_DT_F32> {
   using T = float;
   static __device__ __forceinline__ float f(float v) { return v; }
+  static __device__ __forceinline__ float t(float v) { return v; }
 };
 template <>
 struct In<FP4_DT_BF16> {
   using T = __nv_bfloat16;
   static __device__ __forceinline__ float f(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ __nv_bfloat16 t(float v) { return __float2bfloat16_rn(v); }
 };
 template <>
 struct In<FP4_DT_F16> {
   using T = __half;
   static __device__ __forceinline__ float f(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ __half t(float v) { return __float2half_rn(v); }
 };
 
 template <int DT>
