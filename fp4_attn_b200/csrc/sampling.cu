@@ -5,12 +5,14 @@
 // largest: every sum is then an exact integer sum, the same for any split of a
 // row, and a result depends neither on the grid nor on an order of atomics.
 //
-// A row is read once: a cluster of CTAs holds it in shared memory (up to 16384
-// logits a CTA, in their own type), and everything after that -- the maximum, the sum, the
-// thresholds of top-k and top-p, the draw -- works on chip, with what the CTAs
-// have to tell each other in distributed shared memory.  No sort: a histogram
-// over x finds the bin that the threshold falls into, and only that bin's few
-// logits are ranked.
+// No sort: a histogram over x finds the bin that the threshold of top-k or top-p
+// falls into, and only that bin's few logits are ranked; the draw is a search in
+// the running sums of what is kept, in index order.
+//
+// Few rows: a cluster of CTAs reads a row once and holds it in shared memory; the
+// CTAs exchange their maxima, sums, histograms and the bin's logits over
+// distributed shared memory, and each draws the same conclusions from them.  Many rows: one
+// CTA per row goes over it several times, the later times mostly in L2.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -39,20 +41,21 @@ struct SampleArgs {
   float* logprobs;
 };
 
-// NaN counts as -inf, +inf as the largest finite value.
-__device__ __forceinline__ float sp_clean(float x) { return x != x ? -INFINITY : fminf(x, 3.402823466e38f); }
-
 // Larger keys for larger logits (-0 below +0 would split equal logits: + 0 first).
 __device__ __forceinline__ uint32_t sp_key(float x) {
   const uint32_t b = __float_as_uint(x + 0.0f);
   return (b >> 31) ? ~b : b | 0x80000000u;
 }
 
+__device__ __forceinline__ float logit_of(uint32_t q) { return __uint_as_float(q & 0x80000000u ? q & 0x7fffffffu : ~q); }
+
 constexpr int SP_THREADS = 512, SP_WARPS = SP_THREADS / 32;
-constexpr int SP_BINS = 1024;   // of x's distance from the maximum
+constexpr int SP_BINS = 512;    // of x's distance from the maximum
 constexpr int SP_LIST = 1024;   // logits of a bin that are ranked directly; more of them are searched bit by bit
 constexpr int SP_RANKS = 16;    // CTAs of a cluster
-constexpr int SP_LIMB = 17;     // a weight as two parts of 17 bits: up to 32767 of either add up within 32 bits
+constexpr int SP_LIMB = 17;     // a weight as two parts of 17 bits,
+constexpr int SP_HELD = 32767;  // of which this many add up within 32 bits: logits that a CTA holds
+constexpr float SP_FAR = 3.402823466e38f;
 
 // The last kept logit in the order (x descending, index ascending).
 struct Cut {
@@ -60,28 +63,22 @@ struct Cut {
   int index;
 };
 
-// What the leader (rank 0) tells the cluster to do next.
-enum : int { SP_DONE = 0, SP_GATHER = 1, SP_WIDER = 2, SP_SEARCH = 3 };
-struct Plan {
-  int what, bin, pad[2];
-  Cut cut;
-};
-
-struct SampleShared {
+struct alignas(16) SampleShared {  // (16-byte loads follow it)
   uint32_t count[SP_BINS], lo[SP_BINS], hi[SP_BINS];  // this CTA's histogram
-  // leader: the row's
-  uint32_t total[SP_BINS];
+  uint32_t total[SP_BINS];                            // the row's
   u64 mass[SP_BINS];
-  uint32_t list_key[SP_LIST];
-  int list_index[SP_LIST];
+  u64 list[SP_LIST];  // (key, not index): larger first
   u64 list_w[SP_LIST];
-  int listed;
-  Plan plan;
+  uint32_t mine_key[SP_LIST];  // this CTA's part of the list
+  int mine_index[SP_LIST];
+  int listed, found, last;
+  u64 found_before, last_mass;
+  Cut cut;
   float rank_max[SP_RANKS], rank_min[SP_RANKS];
-  u64 rank_sum[4][SP_RANKS];  // by turns; each slot is written anew only two barriers after it was read
+  u64 rank_sum[4][SP_RANKS];  // by turns; a slot is written anew only several barriers after it was read
   int rank_first[SP_RANKS];
-  u64 warp_sum[SP_WARPS];
-  u64 part[SP_WARPS];
+  u64 part[SP_WARPS], warp_sum[SP_WARPS];
+  int ipart[SP_WARPS];
   float fpart[2][SP_WARPS];
 };
 
@@ -98,50 +95,57 @@ __device__ __forceinline__ T sp_block_sum(T v, T* part) {
   return v;
 }
 
-// The first bin at which the running sum of v (SP_BINS / SP_THREADS bins a thread) reaches `target`, and the sum before
-// it; SP_BINS if it never does.
+// The first bin at which the running sum of v reaches `target`, and the sum before it; SP_BINS if it never does.
 template <typename T>
-__device__ __forceinline__ int sp_find_bin(const T* v, double target, T* part, int* found, u64* before) {
+__device__ __forceinline__ int sp_find_bin(SampleShared& sh, const T* v, double target) {
   constexpr int PER = SP_BINS / SP_THREADS;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  T own[PER], sum = 0;
+  T own[PER];
+  u64 sum = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) sum += own[i] = v[threadIdx.x * PER + i];
-  T inc = sum;
+  u64 inc = sum;
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) {
-    const T u = __shfl_up_sync(0xffffffffu, inc, o);
+    const u64 u = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += u;
   }
   __syncthreads();
-  if (lane == 31) part[warp] = inc;
-  if (threadIdx.x == 0) *found = SP_BINS;
+  if (lane == 31) sh.part[warp] = inc;
+  if (threadIdx.x == 0) sh.found = SP_BINS;
   __syncthreads();
-  T at = inc - sum;
-  for (int i = 0; i < warp; ++i) at += part[i];
+  u64 at = inc - sum;
+#pragma unroll
+  for (int i = 0; i < SP_WARPS; ++i) at += i < warp ? sh.part[i] : 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    if ((double)at < target && (double)(at + own[i]) >= target) *found = threadIdx.x * PER + i, *before = (u64)at;
+    if ((double)at < target && (double)(at + own[i]) >= target) sh.found = threadIdx.x * PER + i, sh.found_before = at;
     at += own[i];
   }
   __syncthreads();
-  return *found;
+  return sh.found;
 }
 
-template <int DT>
-__global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a, int loads) {
+// STREAM: one CTA per row, which reads it anew each time; else a cluster's CTAs hold it.
+template <int DT, bool STREAM>
+__global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a, int loads) {
   using T = typename In<DT>::T;
   constexpr int VEC = 16 / (int)sizeof(T);
   namespace cg = cooperative_groups;
   extern __shared__ __align__(16) uint8_t smem[];
   SampleShared& sh = *reinterpret_cast<SampleShared*>(smem);
+  static_assert(sizeof(SampleShared) % 16 == 0, "what follows is read 16 bytes at a time");
   uint4* held = reinterpret_cast<uint4*>(smem + sizeof(SampleShared));  // [warp][loads][lane]
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  SampleShared& lead = *cluster.map_shared_rank(&sh, 0);
+  const int C = STREAM ? 1 : (int)cluster.num_blocks(), rank = STREAM ? 0 : (int)cluster.block_rank();
+  auto peer = [&](int c) -> SampleShared& { return STREAM ? sh : *cluster.map_shared_rank(&sh, c); };
+  auto barrier = [&]() {
+    if (STREAM || C == 1) __syncthreads();
+    else cluster.sync();
+  };
   const int r = (int)(blockIdx.x / C), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
-  // A warp holds consecutive positions, VEC per lane and load.  Positions count from the 16-byte boundary at or below
+  // A warp has consecutive positions, VEC per lane and load.  Positions count from the 16-byte boundary at or below
   // the row, so that loads are aligned whatever the row's start.
   const T* row = static_cast<const T*>(a.logits) + (int64_t)r * a.ld;
   const int skip = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
@@ -149,40 +153,82 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a, int lo
   const int pos0 = ((rank * SP_WARPS + warp) * loads * 32 + lane) * VEC, end = a.V + skip;
   uint4* mine = held + warp * loads * 32 + lane;  // only this thread's
   const T none = In<DT>::t(-INFINITY);
-#pragma unroll 4
-  for (int j = 0; j < loads; ++j) {
+  auto fetch = [&](int j) {
     const int pos = pos0 + j * 32 * VEC;
     uint4 raw = make_uint4(0u, 0u, 0u, 0u);
     if (pos < end) raw = __ldg(base + pos / VEC);
-    T* t = reinterpret_cast<T*>(&raw);
-    if (pos < skip || pos + VEC > end)
+    if (pos < skip || pos + VEC > end) {
+      T* t = reinterpret_cast<T*>(&raw);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) t[i] = pos + i >= skip && pos + i < end ? t[i] : none;
-    mine[j * 32] = raw;
-  }
-  // calls fn(x, index) for this thread's logits of load j, in order
-  auto load = [&](int j, auto fn) {
-    const uint4 raw = mine[j * 32];
-    const int index = pos0 + j * 32 * VEC - skip;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) fn(sp_clean(In<DT>::f(reinterpret_cast<const T*>(&raw)[i])), index + i);
+    }
+    return raw;
   };
-  auto each = [&](auto fn) {
-#pragma unroll 2
-    for (int j = 0; j < loads; ++j) load(j, fn);
+  // NaN counts as -inf, +inf as the largest finite value.  Where it matters: comparisons pass over NaN by themselves,
+  // and only few logits go further than a comparison.
+  auto clean = [](float v) { return fminf(fmaxf(v, -INFINITY), SP_FAR); };
+  auto value = [&](const uint4& raw, int i) { return In<DT>::f(reinterpret_cast<const T*>(&raw)[i]); };
+  auto index_of = [&](int j) { return pos0 + j * 32 * VEC - skip; };
+  auto load = [&](int j) { return STREAM ? fetch(j) : mine[j * 32]; };
+  // Calls see(x) for each of this thread's logits (not cleaned), and got(x, index) (cleaned) for those that it is true
+  // for.  The hits of up to 16 logits are gathered in a word first: got's code stands once, and the others cost little.
+  constexpr int STEP = STREAM ? 16 / VEC : 8 / VEC;
+  const bool inner = (rank * SP_WARPS + warp) * loads * 32 * VEC >= skip && (rank * SP_WARPS + warp + 1) * loads * 32 * VEC <= end;
+  auto each = [&](auto see, auto got) {
+#pragma unroll 1
+    for (int j = 0; j < loads; j += STEP) {
+      uint4 raw[STEP];
+      if (STREAM && inner && j + STEP <= loads) {
+        const uint4* p = base + (pos0 / VEC + j * 32);
+#pragma unroll
+        for (int i = 0; i < STEP; ++i) raw[i] = __ldg(p + 32 * i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < STEP; ++i) {
+          if (j + i < loads) {
+            raw[i] = load(j + i);
+          } else {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) reinterpret_cast<T*>(&raw[i])[v] = none;
+          }
+        }
+      }
+      uint32_t hits = 0u;
+#pragma unroll
+      for (int i = 0; i < STEP * VEC; ++i) hits |= (see(value(raw[i / VEC], i % VEC)) ? 1u : 0u) << i;
+#pragma unroll 1
+      while (hits) {
+        const int i = __ffs(hits) - 1;
+        hits &= hits - 1;
+        const int at = pos0 + (j + i / VEC) * 32 * VEC + i % VEC;
+        if (j + i / VEC >= loads || at < skip || at >= end) continue;  // what stands in for no logit
+        const T v = STREAM ? __ldg(row + (at - skip)) : reinterpret_cast<const T*>(mine + (j + i / VEC) * 32)[i % VEC];
+        got(clean(In<DT>::f(v)), at - skip);
+      }
+    }
   };
 
   // --------------------------------------------------------- maximum, minimum
-  float mx = -INFINITY, mn = INFINITY;
-  each([&](float v, int) { mx = fmaxf(mx, v), mn = fminf(mn, v == -INFINITY ? INFINITY : v); });
+  if constexpr (!STREAM) {
+#pragma unroll 4
+    for (int j = 0; j < loads; ++j) mine[j * 32] = fetch(j);
+  }
+  for (int i = tid; i < SP_BINS; i += SP_THREADS) sh.count[i] = sh.lo[i] = sh.hi[i] = 0u;
+  if (tid == 0) sh.listed = 0;
+  float mx = -INFINITY, mn = INFINITY;  // mn: of those above -inf
+  each(
+      [&](float v) {
+        mx = fmaxf(mx, v), mn = fminf(mn, v == -INFINITY ? INFINITY : v);
+        return false;
+      },
+      [](float, int) {});
+  mx = fminf(mx, SP_FAR), mn = fminf(mn, SP_FAR);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
   }
   if (lane == 0) sh.fpart[0][warp] = mx, sh.fpart[1][warp] = mn;
-  for (int i = tid; i < SP_BINS; i += SP_THREADS) sh.count[i] = sh.lo[i] = sh.hi[i] = 0u;
-  if (tid == 0) sh.listed = 0;
   __syncthreads();
   if (warp == 0) {
     mx = sh.fpart[0][lane & (SP_WARPS - 1)], mn = sh.fpart[1][lane & (SP_WARPS - 1)];
@@ -191,12 +237,9 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a, int lo
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
       mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
     }
-    if (lane < C) {  // to every CTA
-      SampleShared& to = *cluster.map_shared_rank(&sh, lane);
-      to.rank_max[rank] = mx, to.rank_min[rank] = mn;
-    }
+    if (lane < C) peer(lane).rank_max[rank] = mx, peer(lane).rank_min[rank] = mn;
   }
-  cluster.sync();
+  barrier();
   mx = sh.rank_max[0], mn = sh.rank_min[0];
   for (int i = 1; i < C; ++i) mx = fmaxf(mx, sh.rank_max[i]), mn = fminf(mn, sh.rank_min[i]);
   if (mx == -INFINITY) {  // the same in every CTA
@@ -215,59 +258,119 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a, int lo
   const double f = 1.4426950408889634 / (double)temp;
   const float f1 = (float)f, f2 = (float)(f - (double)f1);
   auto weight = [&](float v) -> u64 {
-    const float d = v - mx;
-    float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaxf(fmaf(d, f1, d * f2), -150.0f)));  // (NaN: both parts infinite)
-    return v == -INFINITY ? 0ull : __float2ull_rn(e * SP_ONE);
+    const float d = fminf(v, SP_FAR) - mx;
+    float e;  // (a NaN or an infinite d gives NaN or -inf, and so 0)
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaxf(fmaf(d, f1, d * f2), -150.0f)));
+    return __float2ull_rn(e * SP_ONE);  // (2^34 in the exponent's argument would cost it four bits)
   };
   int turn = 0;
   // The cluster's sum of a number per thread.
-  auto cluster_sum = [&](u64 v) -> u64 {
+  auto row_sum = [&](u64 v) -> u64 {
     v = sp_block_sum(v, sh.part);
-    if (tid < C) cluster.map_shared_rank(&sh, tid)->rank_sum[turn & 3][rank] = v;
-    cluster.sync();
+    if (tid < C) peer(tid).rank_sum[turn & 3][rank] = v;
+    barrier();
     u64 sum = 0;
     for (int i = 0; i < C; ++i) sum += sh.rank_sum[turn & 3][i];
     ++turn;
     return sum;
   };
+  // The sum of what comes before this warp, in index order, and the row's; `own`: this thread's.
+  struct Before {
+    u64 before, warp, total;
+  };
+  auto row_scan = [&](u64 own) -> Before {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) own += __shfl_xor_sync(0xffffffffu, own, o);
+    __syncthreads();
+    if (lane == 0) sh.warp_sum[warp] = own;
+    __syncthreads();
+    u64 block = 0;
+    Before s{0, own, 0};
+#pragma unroll
+    for (int i = 0; i < SP_WARPS; ++i) {
+      block += sh.warp_sum[i];
+      if (i < warp) s.before += sh.warp_sum[i];
+    }
+    if (tid < C) peer(tid).rank_sum[turn & 3][rank] = block;
+    barrier();
+    for (int i = 0; i < C; ++i) {
+      if (i < rank) s.before += sh.rank_sum[turn & 3][i];
+      s.total += sh.rank_sum[turn & 3][i];
+    }
+    ++turn;
+    return s;
+  };
+  // Calls hit(x, index) for the logit at which the running sum of fn(x, index) passes `target`, in its warp.
+  auto row_find = [&](const Before& s, u64 target, auto fn, auto hit) {
+    if (!(s.before <= target && target < s.before + s.warp)) return;
+    u64 before = s.before;
+#pragma unroll 1
+    for (int j = 0; j < loads; ++j) {
+      const uint4 raw = load(j);
+      u64 here = 0;
+#pragma unroll 1
+      for (int i = 0; i < VEC; ++i) here += fn(clean(value(raw, i)), index_of(j) + i);
+      u64 inc = here;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const u64 u = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += u;
+      }
+      u64 at = before + inc - here;
+      if (at <= target && target < at + here)
+#pragma unroll 1
+        for (int i = 0; i < VEC; ++i) {
+          const float v = clean(value(raw, i));
+          const u64 w = fn(v, index_of(j) + i);
+          if (at <= target && target < at + w) hit(v, index_of(j) + i);
+          at += w;
+        }
+      before += __shfl_sync(0xffffffffu, inc, 31);
+      if (before > target) break;
+    }
+  };
 
-  // ------------------------------------------------- sum, first largest logit
+  // ------------------------------- sum, first largest logit, first histogram
+  // of what can hold the thresholds: first the logits within 6 (or 6 T) of the maximum, which are few and mostly
+  // enough; a logit in the histogram costs as much as three that are only summed, a second histogram a pass over the row
+  const float full = fminf(24.6f * temp, mx - mn);  // weights further away are 0
+  const float near = full <= 8.0f ? full : fminf(fmaxf(6.0f * temp, 6.0f), full);
+  float from = -1.0f, reach = near, per = reach > 0.0f ? (float)SP_BINS / reach : 0.0f;  // the band (from, reach] below mx
+  auto in_band = [&](float v) { return mx - v > from && mx - v <= reach; };
+  auto bin_of = [&](float v) { return max(0, min(SP_BINS - 1, (int)((mx - v - fmaxf(from, 0.0f)) * per))); };
+  auto add = [&](float v) {
+    const int b = bin_of(v);
+    const u64 w = weight(v);
+    atomicAdd(&sh.count[b], 1u);
+    atomicAdd(&sh.lo[b], (uint32_t)w & ((1u << SP_LIMB) - 1));
+    atomicAdd(&sh.hi[b], (uint32_t)(w >> SP_LIMB));
+  };
   u64 z = 0;
   int first = INT32_MAX;
-  each([&](float v, int index) {
-    z += weight(v);
-    if (v == mx) first = min(first, index);
-  });
-  first = __reduce_min_sync(0xffffffffu, first);
-  if (lane == 0) sh.list_index[warp] = first;  // (the list is not in use yet)
-  z = sp_block_sum(z, sh.part);
-  if (tid < C) {
-    int m = INT32_MAX;
-    for (int i = 0; i < SP_WARPS; ++i) m = min(m, sh.list_index[i]);
-    SampleShared& to = *cluster.map_shared_rank(&sh, tid);
-    to.rank_sum[3][rank] = z, to.rank_first[rank] = m;
+  {
+    // hits: what the histogram takes, or a greedy row's largest
+    const float low = greedy ? mx : by_k || by_p ? mx - reach : INFINITY;
+    each(
+        [&](float v) {
+          z += weight(v);
+          return v >= low;
+        },
+        [&](float v, int index) {
+          if (greedy) first = min(first, index);
+          else if (in_band(v)) add(v);
+        });
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0) sh.ipart[warp] = first;
+    z = sp_block_sum(z, sh.part);
+    if (tid < C) {
+      int m = INT32_MAX;
+#pragma unroll
+      for (int i = 0; i < SP_WARPS; ++i) m = min(m, sh.ipart[i]);
+      peer(tid).rank_sum[3][rank] = z, peer(tid).rank_first[rank] = m;
+    }
   }
-  // the histogram of what can hold the thresholds: first the logits within 10 T of the maximum
-  const float full = fminf(24.6f * temp, mx - mn);  // weights further away are 0
-  float reach = fminf(10.0f * temp, full);
-  auto bin_of = [&](float v, float per) { return min(SP_BINS - 1, (int)((mx - v) * per)); };
-  auto histogram = [&](float per) {
-    each([&](float v, int) {
-      if (mx - v <= reach) {
-        const int b = bin_of(v, per);
-        const u64 w = weight(v);
-        atomicAdd(&sh.count[b], 1u);
-        atomicAdd(&sh.lo[b], (uint32_t)w & ((1u << SP_LIMB) - 1));
-        atomicAdd(&sh.hi[b], (uint32_t)(w >> SP_LIMB));
-      }
-    });
-  };
-  float per = reach > 0.0f ? (float)SP_BINS / reach : 0.0f;
-  if (by_k || by_p) histogram(per);
-  cluster.sync();
-  z = 0;
-  first = INT32_MAX;
+  barrier();
+  z = 0, first = INT32_MAX;
   for (int i = 0; i < C; ++i) z += sh.rank_sum[3][i], first = min(first, sh.rank_first[i]);
   const float logz = logf((float)((double)z / (double)SP_ONE));
   if (greedy) {
@@ -275,153 +378,177 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a, int lo
       a.tokens[r] = first;
       if (a.logprobs) a.logprobs[r] = -logz;
     }
-    cluster.sync();  // no CTA leaves while another may still write to it
-    return;
+    return;  // (the barrier above was behind the last access to another CTA)
   }
 
   Cut cut{0u, INT32_MAX};
-  // Kept so far: everything down to the cut.
-  auto within = [&](uint32_t q, int index) { return q > cut.key || (q == cut.key && index <= cut.index); };
-
+  bool search = false;
   // what has to go before a logit for top_p to drop it; the first always stays
   auto p_target = [&](u64 mass) { return fmax((double)top_p * (double)mass, 1.0); };
-
   if (by_k || by_p) {
-    bool k_done = !by_k;  // the leader's: top_k is settled
-    u64 kept_mass = z;    // and what it leaves
-    for (;;) {
-      // the row's histogram, a share of the bins per CTA
-      const int share = SP_BINS / C;
-      for (int i = rank * share + tid; i < (rank + 1) * share; i += SP_THREADS) {
+    // Every CTA has the row's whole histogram and, of the bin it then needs, all logits: all of them come to the same cut.
+    auto merge = [&]() -> bool {
+      bool fine = true;
+      for (int i = tid; i < SP_BINS; i += SP_THREADS) {
         uint32_t n = 0;
         u64 lo = 0, hi = 0;
-        for (int c = 0; c < C; ++c) {
-          const SampleShared& from = *cluster.map_shared_rank(&sh, c);
-          n += from.count[i], lo += from.lo[i], hi += from.hi[i];
-        }
-        lead.total[i] = n, lead.mass[i] = lo + (hi << SP_LIMB);
-      }
-      cluster.sync();
-      // the leader finds the bin
-      auto choose = [&]() {
-        __shared__ int found;
-        __shared__ u64 before;
-        Plan p{SP_DONE, 0, {0, 0}, cut};
-        int b = SP_BINS;
-        if (!k_done) {
-          b = sp_find_bin(sh.total, (double)k, reinterpret_cast<uint32_t*>(sh.part), &found, &before);
-          if (b == SP_BINS && reach < full) {
-            p.what = SP_WIDER;
-            return p;
-          }
-          if (b == SP_BINS) k_done = true;  // fewer than k weights are not 0
-        }
-        if (k_done) {
-          if (!by_p) return p;
-          b = sp_find_bin(sh.mass, p_target(kept_mass), sh.part, &found, &before);
-        }
-        // (the full reach has all of the mass)
-        if (b == SP_BINS) p.what = reach < full ? SP_WIDER : SP_SEARCH;
-        else p.what = sh.total[b] <= SP_LIST ? SP_GATHER : SP_SEARCH, p.bin = b;
-        return p;
-      };
-      auto tell = [&](const Plan& p) {
-        if (tid < C) cluster.map_shared_rank(&sh, tid)->plan = p;
-        if (tid == 0) sh.listed = 0;
-      };
-      if (rank == 0) tell(choose());
-      cluster.sync();
-      while (sh.plan.what == SP_GATHER) {
-        const int bin = sh.plan.bin;
-        each([&](float v, int index) {
-          if (mx - v <= reach && bin_of(v, per) == bin) {
-            const int at = atomicAdd(&lead.listed, 1);
-            if (at < SP_LIST) lead.list_key[at] = sp_key(v), lead.list_index[at] = index, lead.list_w[at] = weight(v);
-          }
-        });
-        cluster.sync();
-        if (rank == 0) {
-          // rank the listed ones: how many, and how much, goes before each
-          const int n = min(sh.listed, SP_LIST);
-          u64 above_n = 0, above_w = 0;
-          for (int i = tid; i < bin; i += SP_THREADS) above_n += sh.total[i], above_w += sh.mass[i];
-          above_n = sp_block_sum(above_n, sh.part), above_w = sp_block_sum(above_w, sh.part);
-          int at_n[SP_LIST / SP_THREADS];
-          u64 at_w[SP_LIST / SP_THREADS];
+        for (int c0 = 0; c0 < C; c0 += 8) {  // (eight CTAs' at a time: a trip over the cluster takes long)
+          uint32_t m[8], l[8], h[8];
 #pragma unroll
-          for (int t = 0; t < SP_LIST / SP_THREADS; ++t) {
-            const int e = tid + t * SP_THREADS;
-            at_n[t] = 0, at_w[t] = 0;
-            if (e < n) {
-              const uint32_t q = sh.list_key[e];
-              const int id = sh.list_index[e];
-              for (int i = 0; i < n; ++i)
-                if (sh.list_key[i] > q || (sh.list_key[i] == q && sh.list_index[i] < id)) ++at_n[t], at_w[t] += sh.list_w[i];
+          for (int c = 0; c < 8; ++c) {
+            const SampleShared& from = peer(min(c0 + c, C - 1));
+            m[c] = from.count[i], l[c] = from.lo[i], h[c] = from.hi[i];
+          }
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            if (c0 + c < C) {
+              fine = fine && m[c] <= SP_HELD;  // more may have run over (a row that is read anew)
+              n += m[c], lo += l[c], hi += h[c];
             }
-          }
-          // the last one kept is the one with the most kept ones before it
-          __shared__ int last;
-          auto settle = [&](auto keeps) {
-            __syncthreads();
-            if (tid == 0) last = -1;
-            __syncthreads();
-#pragma unroll
-            for (int t = 0; t < SP_LIST / SP_THREADS; ++t)
-              if (tid + t * SP_THREADS < n && keeps(t)) atomicMax(&last, at_n[t]);
-            __syncthreads();
-#pragma unroll
-            for (int t = 0; t < SP_LIST / SP_THREADS; ++t)
-              if (tid + t * SP_THREADS < n && at_n[t] == last) {
-                sh.plan.cut = {sh.list_key[tid + t * SP_THREADS], sh.list_index[tid + t * SP_THREADS]};
-                sh.part[0] = above_w + at_w[t] + sh.list_w[tid + t * SP_THREADS];
-              }
-            __syncthreads();
-            cut = sh.plan.cut;
-            const u64 mass = sh.part[0];
-            __syncthreads();
-            return mass;
-          };
-          if (!k_done) {
-            kept_mass = settle([&](int t) { return above_n + at_n[t] < (u64)k; });
-            k_done = true;
-            if (by_p) {
-              Plan p = choose();
-              // (the mass up to the cut reaches the target, so the bin is this one or an earlier one)
-              if (p.what == SP_GATHER && p.bin == bin) {
-                const double target = p_target(kept_mass);
-                settle([&](int t) { return above_n + at_n[t] < (u64)k && (double)(above_w + at_w[t]) < target; });
-                p.what = SP_DONE, p.cut = cut;
-              }
-              tell(p);
-            } else {
-              tell({SP_DONE, 0, {0, 0}, cut});
-            }
-          } else {
-            const double target = p_target(kept_mass);
-            settle([&](int t) { return (double)(above_w + at_w[t]) < target; });
-            tell({SP_DONE, 0, {0, 0}, cut});
-          }
         }
-        cluster.sync();
+        sh.total[i] = n, sh.mass[i] = lo + (hi << SP_LIMB);
       }
-      cut = sh.plan.cut;
-      if (sh.plan.what != SP_WIDER) break;
-      reach = full, per = (float)SP_BINS / reach;
-      cluster.sync();  // (the histograms have been read)
+      return __syncthreads_and(fine);
+    };
+    u64 base_n = 0, base_w = 0;  // above the band
+    bool merged = merge();
+    // another band's histogram; false if it cannot be had
+    auto band = [&](float lo, float hi) -> bool {
+      from = lo, reach = hi, per = (float)SP_BINS / (reach - fmaxf(from, 0.0f));
+      barrier();  // (the histograms have been read)
       for (int i = tid; i < SP_BINS; i += SP_THREADS) sh.count[i] = sh.lo[i] = sh.hi[i] = 0u;
       __syncthreads();
-      histogram(per);
-      cluster.sync();
+      const float upper = from < 0.0f ? INFINITY : mx - from + fabsf(mx) * 2.4e-7f, lower = mx - reach - fabsf(mx) * 2.4e-7f;
+      each([&](float v) { return v >= lower && v <= upper; },
+           [&](float v, int) {
+             if (in_band(v)) add(v);
+           });
+      barrier();
+      return merge();
+    };
+    // the bin where the count, or the mass, reaches the target, in this band or one further away; SP_BINS: nowhere
+    auto locate = [&](bool by_mass, double target) -> int {
+      for (;;) {
+        const int b = by_mass ? sp_find_bin(sh, sh.mass, target - (double)base_w) : sp_find_bin(sh, sh.total, target - (double)base_n);
+        if (b < SP_BINS || reach >= full) return b;
+        u64 sn = 0, sw = 0;
+        for (int i = tid; i < SP_BINS; i += SP_THREADS) sn += sh.total[i], sw += sh.mass[i];
+        base_n += sp_block_sum(sn, sh.part), base_w += sp_block_sum(sw, sh.part);
+        if (!(merged = merged && band(reach, fminf(full, reach * 1.3f)))) return SP_BINS;
+      }
+    };
+    int listed_bin = -1, n = 0;
+    u64 above_n = 0, above_w = 0;
+    int at_n[SP_LIST / SP_THREADS];
+    u64 at_w[SP_LIST / SP_THREADS];
+    // the bin's logits, and how many and how much goes before each of this thread's
+    auto list = [&](int bin) {
+      if (listed_bin >= 0) {
+        barrier();  // (the last list has been read)
+        if (tid == 0) sh.listed = 0;
+        barrier();
+      }
+      listed_bin = bin;
+      // (a range that surely has the bin, to pass over the others quickly)
+      const float wide = fabsf(mx) * 2.4e-7f, at0 = mx - fmaxf(from, 0.0f);
+      const float hi = bin ? at0 - (float)(bin - 1) / per + wide : INFINITY;
+      const float lo = per > 0.0f ? at0 - (float)(bin + 2) / per - wide : -INFINITY;
+      each([&](float v) { return v >= lo && v <= hi; },
+           [&](float v, int index) {
+             if (in_band(v) && bin_of(v) == bin) {
+               const int at = atomicAdd(&sh.listed, 1);
+               if (at < SP_LIST) sh.mine_key[at] = sp_key(v), sh.mine_index[at] = index;
+             }
+           });
+      barrier();
+      // everybody's, one after the other
+      if (tid < C) sh.rank_first[tid] = peer(tid).listed;
+      __syncthreads();
+      n = 0;
+      for (int c = 0; c < C; ++c) n += sh.rank_first[c];
+      n = min(n, SP_LIST);
+      for (int e = tid; e < n; e += SP_THREADS) {
+        int c = 0, i = e;
+        while (i >= sh.rank_first[c]) i -= sh.rank_first[c++];
+        const uint32_t q = peer(c).mine_key[i];
+        sh.list[e] = (u64)q << 32 | (uint32_t)~peer(c).mine_index[i], sh.list_w[e] = weight(logit_of(q));
+      }
+      __syncthreads();
+      u64 sn = 0, sw = 0;
+      for (int i = tid; i < bin; i += SP_THREADS) sn += sh.total[i], sw += sh.mass[i];
+      above_n = base_n + sp_block_sum(sn, sh.part), above_w = base_w + sp_block_sum(sw, sh.part);
+#pragma unroll
+      for (int t = 0; t < SP_LIST / SP_THREADS; ++t) {
+        const int e = tid + t * SP_THREADS;
+        at_n[t] = 0, at_w[t] = 0;
+        if (e < n) {
+          const u64 own = sh.list[e];
+#pragma unroll 4
+          for (int i = 0; i < n; ++i) {
+            const bool ahead = sh.list[i] > own;
+            at_n[t] += ahead, at_w[t] += ahead ? sh.list_w[i] : 0ull;
+          }
+        }
+      }
+    };
+    // the cut behind the listed logits that keeps(t) holds for, and the mass down to it
+    auto settle = [&](auto keeps) -> u64 {
+      __syncthreads();
+      if (tid == 0) sh.last = -1;
+      __syncthreads();
+#pragma unroll
+      for (int t = 0; t < SP_LIST / SP_THREADS; ++t)
+        if (tid + t * SP_THREADS < n && keeps(t)) atomicMax(&sh.last, at_n[t]);
+      __syncthreads();
+#pragma unroll
+      for (int t = 0; t < SP_LIST / SP_THREADS; ++t) {
+        const int e = tid + t * SP_THREADS;
+        if (e < n && at_n[t] == sh.last) {
+          sh.cut = {(uint32_t)(sh.list[e] >> 32), (int)~(uint32_t)sh.list[e]};
+          sh.last_mass = above_w + at_w[t] + sh.list_w[e];
+        }
+      }
+      __syncthreads();
+      cut = sh.cut;
+      return sh.last_mass;
+    };
+    u64 mass = z;  // what is kept so far
+    if (by_k && merged) {
+      const int b = locate(false, (double)k);
+      if (b < SP_BINS && merged) {  // (else fewer than k weights are not 0)
+        if (sh.total[b] > SP_LIST) search = true;
+        else list(b), mass = settle([&](int t) { return above_n + at_n[t] < (u64)k; });
+      }
     }
-    if (sh.plan.what == SP_SEARCH) {
-      // Too many logits in one bin (flat rows): the thresholds bit by bit, on the logits in registers.
+    if (by_p && merged && !search) {
+      const double target = p_target(mass);
+      if ((double)base_w >= target) {  // top_k went past the band that has it
+        base_n = base_w = 0;
+        listed_bin = SP_BINS;
+        merged = band(-1.0f, near);
+      }
+      const int b = merged ? locate(true, target) : SP_BINS;
+      if (b == SP_BINS || sh.total[b] > SP_LIST) {
+        search = true;
+      } else {
+        if (b != listed_bin) list(b);
+        // (what top_k dropped has all of `mass` before it, more than the target)
+        settle([&](int t) { return (double)(above_w + at_w[t]) < target; });
+      }
+    }
+    search = search || !merged;
+    if (search) {
+      // Too many logits in one bin (flat rows): the thresholds bit by bit.
       cut = {0u, INT32_MAX};
       auto above = [&](uint32_t q, bool by_mass) {
         u64 s = 0;
-        each([&](float v, int) {
-          if (v != -INFINITY && sp_key(v) > q) s += by_mass ? weight(v) : 1ull;
-        });
-        return cluster_sum(s);
+        each(
+            [&](float v) {
+              if (v > -INFINITY && sp_key(clean(v)) > q) s += by_mass ? weight(v) : 1ull;
+              return false;
+            },
+            [](float, int) {});
+        return row_sum(s);
       };
       auto largest = [&](bool by_mass, double target) {  // the largest key whose own and larger ones reach the target
         uint32_t lo = 0;
@@ -432,150 +559,95 @@ __global__ void __launch_bounds__(SP_THREADS) sample_kernel(SampleArgs a, int lo
         }
         return lo;
       };
-      // the index of the n-th (from 0) logit of key q
+      // the cut at the n-th (from 0) logit of key q
       auto nth = [&](uint32_t q, u64 n) {
+        auto is = [&](float v, int) -> u64 { return v != -INFINITY && sp_key(v) == q; };
         u64 own = 0;
-        each([&](float v, int) { own += v != -INFINITY && sp_key(v) == q; });
-        // before this warp: in lower CTAs and lower warps
-        u64 w = own;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-        __syncthreads();
-        if (lane == 0) sh.warp_sum[warp] = w;
-        __syncthreads();
-        u64 block = 0, before = 0;
-        for (int i = 0; i < SP_WARPS; ++i) block += sh.warp_sum[i], before += i < warp ? sh.warp_sum[i] : 0;
-        if (tid < C) cluster.map_shared_rank(&sh, tid)->rank_sum[turn & 3][rank] = block;
-        cluster.sync();
-        for (int i = 0; i < rank; ++i) before += sh.rank_sum[turn & 3][i];
-        ++turn;
-        if (before <= n && n < before + w) {
-          for (int j = 0; j < loads; ++j) {
-            u64 here = 0;
-            load(j, [&](float v, int) { here += v != -INFINITY && sp_key(v) == q; });
-            u64 inc = here;
-#pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-              const u64 u = __shfl_up_sync(0xffffffffu, inc, o);
-              if (lane >= o) inc += u;
-            }
-            u64 at = before + inc - here;
-            load(j, [&](float v, int index) {
-              if (v != -INFINITY && sp_key(v) == q) {
-                if (at == n)
-                  for (int c = 0; c < C; ++c) cluster.map_shared_rank(&sh, c)->plan.cut = {q, index};
-                ++at;
-              }
-            });
-            before += __shfl_sync(0xffffffffu, inc, 31);
-          }
-        }
-        cluster.sync();
-        const Cut found = sh.plan.cut;
-        cluster.sync();
-        return found;
+        each([&](float v) { return v > -INFINITY && sp_key(clean(v)) == q; }, [&](float v, int index) { own += is(v, index); });
+        row_find(row_scan(own), n, is, [&](float, int index) {
+          for (int c = 0; c < C; ++c) peer(c).cut = {q, index};
+        });
+        barrier();
+        const Cut c = sh.cut;
+        barrier();
+        return c;
       };
-      auto key_weight = [&](uint32_t q) { return weight(__uint_as_float(q & 0x80000000u ? q & 0x7fffffffu : ~q)); };
-      u64 mass = z;
-      if (by_k) {
-        const u64 all = above(0u, false);
-        if (all > (u64)k) {
-          const uint32_t q = largest(false, (double)k);
-          const u64 more = above(q, false);
-          mass = above(q, true) + ((u64)k - more) * key_weight(q);
-          cut = nth(q, (u64)k - more - 1);
-        }
+      auto key_weight = [&](uint32_t q) { return weight(logit_of(q)); };
+      mass = z;
+      if (by_k && above(0u, false) > (u64)k) {
+        const uint32_t q = largest(false, (double)k);
+        const u64 more = above(q, false);
+        mass = above(q, true) + ((u64)k - more) * key_weight(q);
+        cut = nth(q, (u64)k - more - 1);
       }
       if (by_p) {
         const double target = p_target(mass);
         const uint32_t q = max(largest(true, target), cut.key);
         const u64 before = above(q, true), w = key_weight(q);
         // how many of key q have less than the target before them
-        u64 n = 0;
-        if (w > 0) {
-          u64 lo = 0, hi = (u64)a.V;
-          while (lo < hi) {
-            const u64 mid = (lo + hi) / 2;
-            if ((double)(before + mid * w) < target) lo = mid + 1; else hi = mid;
-          }
-          n = lo;
+        u64 lo = 0, hi = w > 0 ? (u64)a.V : 0;
+        while (lo < hi) {
+          const u64 mid = (lo + hi) / 2;
+          if ((double)(before + mid * w) < target) lo = mid + 1;
+          else hi = mid;
         }
-        // none: the target is 0, or reached before q by the cut that top_k made
-        if (n > 0) {
-          const Cut c2 = nth(q, min(n, above(q - 1, false) - above(q, false)) - 1);
-          if (c2.key > cut.key || (c2.key == cut.key && c2.index < cut.index)) cut = c2;
-        } else if (before == 0) {
-          cut = {sp_key(mx), first};
+        if (lo > 0) {  // (else q is where top_k cut, and the target is reached before it)
+          const Cut c = nth(q, min(lo, above(q - 1, false) - above(q, false)) - 1);
+          if (c.key > cut.key || (c.key == cut.key && c.index < cut.index)) cut = c;
         }
       }
     }
-    if (cut.key > sp_key(mx) || (cut.key == sp_key(mx) && cut.index < first)) cut = {sp_key(mx), first};
   }
 
   // ----------------------------------------------------------------- the draw
-  const double least = (double)fminf(min_p, 1.0f) * (double)SP_ONE;
+  const u64 least = (u64)ceil((double)fmaxf(fminf(min_p, 1.0f), 0.0f) * (double)SP_ONE);
+  // (key 0 is below every logit's)
+  const float edge = cut.key == 0u ? -INFINITY : logit_of(cut.key);
   auto kept = [&](float v, int index) -> u64 {
-    if (v == -INFINITY || !within(sp_key(v), index)) return 0ull;
+    if (!(v > edge || (v == edge && index <= cut.index))) return 0ull;
     const u64 w = weight(v);
-    return (double)w >= least ? w : 0ull;
+    return w >= least ? w : 0ull;
   };
   u64 own = 0;
-  each([&](float v, int index) { own += kept(v, index); });
-  u64 w = own;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-  __syncthreads();
-  if (lane == 0) sh.warp_sum[warp] = w;
-  __syncthreads();
-  u64 block = 0, before = 0;
-  for (int i = 0; i < SP_WARPS; ++i) block += sh.warp_sum[i], before += i < warp ? sh.warp_sum[i] : 0;
-  if (tid < C) cluster.map_shared_rank(&sh, tid)->rank_sum[turn & 3][rank] = block;
-  cluster.sync();  // the last access to another CTA's memory is behind this barrier
-  u64 total = 0;
-  for (int i = 0; i < C; ++i) {
-    const u64 s = sh.rank_sum[turn & 3][i];
-    total += s;
-    if (i < rank) before += s;
+  if (cut.key == 0u) {
+    each(
+        [&](float v) {
+          const u64 w = weight(v);
+          own += w >= least ? w : 0ull;
+          return false;
+        },
+        [](float, int) {});
+  } else {
+    each([&](float v) { return v >= edge; }, [&](float v, int index) { own += kept(v, index); });
   }
-  const u64 target = min((u64)floor((double)a.u[r] * (double)total), total - 1);
-  if (before <= target && target < before + w) {
-    // this warp has it
-    for (int j = 0; j < loads; ++j) {
-      u64 here = 0;
-      load(j, [&](float v, int index) { here += kept(v, index); });
-      u64 inc = here;
-#pragma unroll
-      for (int o = 1; o < 32; o *= 2) {
-        const u64 u = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += u;
-      }
-      u64 at = before + inc - here;
-      if (at <= target && target < at + here)
-        load(j, [&](float v, int index) {
-          const u64 w1 = kept(v, index);
-          if (at <= target && target < at + w1) {
-            a.tokens[r] = index;
-            if (a.logprobs) a.logprobs[r] = (v - mx) / temp - logz;
-          }
-          at += w1;
-        });
-      before += __shfl_sync(0xffffffffu, inc, 31);
-    }
-  }
+  const Before s = row_scan(own);  // its barrier is behind the last access to another CTA's memory
+  const u64 target = min((u64)floor((double)a.u[r] * (double)s.total), s.total - 1);
+  row_find(s, target, kept, [&](float v, int index) {
+    a.tokens[r] = index;
+    if (a.logprobs) a.logprobs[r] = (v - mx) / temp - logz;
+  });
 }
 
-// CTAs of a row's cluster: enough for 16384 logits each (and a load more where the row is not aligned), more
-// where rows are few: the card has 148 SMs, and a row's time is that of its slowest CTA.
+// Many rows, one CTA each: its time is its instructions (about 35 a logit), and no CTA waits for another.  Few rows: a
+// cluster of CTAs each, as many as fill the card's 2 x 148 places but at most 8 unless the row needs more, since every
+// exchange over the cluster costs about a microsecond.
 template <int DT>
 int launch_sample(const SampleArgs& a, cudaStream_t st) {
   constexpr int VEC = DT == FP4_DT_F32 ? 4 : 8;
-  const int n = a.V + VEC - 1;  // a row can begin VEC - 1 logits past a 16-byte boundary
+  // a row can begin VEC - 1 logits past a 16-byte boundary
+  const bool aligned = (uintptr_t)a.logits % 16 == 0 && (a.ld % VEC == 0 || a.R == 1);
+  const int n = a.V + (aligned ? 0 : VEC - 1);
+  const int most = DT == FP4_DT_F32 ? 16384 : 28672;  // 64 or 56 KB: two CTAs on an SM
   int C = 1;
-  while (C < SP_RANKS && C * 16384 < n) C *= 2;
-  while (C < 8 && (int64_t)a.R * C < 148 && C * 4096 < n) C *= 2;
+  while (C < SP_RANKS && C * most < n) C *= 2;
+  const bool stream = C > 1 && (int64_t)a.R * C > 296;
+  if (stream) C = 1;
+  else
+    while (C < 8 && (int64_t)a.R * C * 2 <= 296 && C * 4096 < n) C *= 2;
   const int per_load = C * SP_THREADS * VEC, loads = (n + per_load - 1) / per_load;
-  const size_t smem = sizeof(SampleShared) + (size_t)loads * SP_THREADS * 16;
-  if (int e = set_smem_attr((const void*)sample_kernel<DT>, (int)(sizeof(SampleShared) + 65536 + SP_THREADS * 16), true)) return e;
+  const size_t smem = sizeof(SampleShared) + (stream ? 0 : (size_t)loads * SP_THREADS * 16);
+  auto* fn = stream ? sample_kernel<DT, true> : sample_kernel<DT, false>;
+  if (int e = set_smem_attr((const void*)fn, (int)sizeof(SampleShared) + 73728, true)) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.R * C)), cfg.blockDim = dim3(SP_THREADS);
   cfg.dynamicSmemBytes = smem, cfg.stream = st;
@@ -583,7 +655,7 @@ int launch_sample(const SampleArgs& a, cudaStream_t st) {
   at.id = cudaLaunchAttributeClusterDimension;
   at.val.clusterDim.x = (unsigned)C, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
   cfg.attrs = &at, cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, sample_kernel<DT>, a, loads);
+  cudaLaunchKernelEx(&cfg, fn, a, loads);
   return check_launch("sample_kernel");
 }
 
