@@ -106,6 +106,11 @@ def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+def raw_stream(device_index: int) -> int:
+    """The same by device index, without making a Stream object (2 us of a small call)."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
+
+
 def require_cuda(*tensors: torch.Tensor) -> None:
     for t in tensors:
         if not t.is_cuda:

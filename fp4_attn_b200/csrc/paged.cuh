@@ -76,9 +76,10 @@ __device__ __forceinline__ uint32_t pg_block(const Blk& x, float r, uint2& codes
 
 // A warp quantizes one token of H heads: lane l takes blocks l, l + 32, ...; at(block) is where the block's
 // elements are, put(block, codes, scale) stores it.  Returns the token's g.  Up to NB blocks a lane stay in
-// registers between the maximum and the codes (NB 0: read twice).
-template <int DT, bool VEC, int NB, typename At, typename Put>
-__device__ __forceinline__ float pg_quantize_token(int nblk, At at, Put put) {
+// registers between the maximum and the codes (NB 0: read twice).  where() finds the token's place, while its loads
+// are on their way; if it has none (false), nothing is stored.
+template <int DT, bool VEC, int NB, typename At, typename Where, typename Put>
+__device__ __forceinline__ float pg_quantize_token(int nblk, At at, Where where, Put put) {
   const int lane = threadIdx.x & 31;
   float m = 0.0f, r;
   if constexpr (NB > 0) {
@@ -86,6 +87,7 @@ __device__ __forceinline__ float pg_quantize_token(int nblk, At at, Put put) {
 #pragma unroll
     for (int i = 0; i < NB; ++i)
       if (lane + 32 * i < nblk) x[i].load(at(lane + 32 * i));
+    if (!where()) return 0.0f;
 #pragma unroll
     for (int i = 0; i < NB; ++i)
       if (lane + 32 * i < nblk) m = nanmax(m, x[i].absmax());
@@ -101,6 +103,7 @@ __device__ __forceinline__ float pg_quantize_token(int nblk, At at, Put put) {
       }
     return g;
   } else {
+    if (!where()) return 0.0f;
     Block16<DT, VEC> x;
     for (int i = lane; i < nblk; i += 32) x.load(at(i)), m = nanmax(m, x.absmax());
 #pragma unroll

@@ -174,22 +174,30 @@ __global__ void __launch_bounds__(256) append_quant_kernel(fp4paged_cache c, con
   if (id >= (int64_t)a.B * a.T) return;
   const int b = (int)(id / a.T), t = (int)(id % a.T);
   const Work w = work_of(c);
-  if (t >= w.count[b]) return;
-  const int pos = w.start[b] + t;
-  const int64_t page = c.page_table[(int64_t)pg_seq(c, seqs, b) * c.max_pages + pos / P];
-  const int slot = pos % P;
   const E* x = static_cast<const E*>(a.x[kv]) + b * a.sB[kv] + t * a.sT[kv];
   const int64_t sH = a.sH[kv];
-  uint8_t* codes = (kv ? c.v_codes : c.k_codes) + (page * H * P + slot) * PG_ROW;
-  uint8_t* scales = (kv ? c.v_scales : c.k_scales) + (page * H * P + slot) * PG_SF;
+  int64_t page = 0;
+  int slot = 0;
+  uint8_t *codes = nullptr, *scales = nullptr;
+  bool live = false;
   const float g = pg_quantize_token<DT, VEC, NB>(
       H * PG_SF, [&](int i) { return x + (i >> 3) * sH + (i & 7) * 16; },
+      [&]() {
+        live = t < w.count[b];
+        if (!live) return false;
+        const int pos = w.start[b] + t;
+        page = c.page_table[(int64_t)pg_seq(c, seqs, b) * c.max_pages + pos / P];
+        slot = pos % P;
+        codes = (kv ? c.v_codes : c.k_codes) + (page * H * P + slot) * PG_ROW;
+        scales = (kv ? c.v_scales : c.k_scales) + (page * H * P + slot) * PG_SF;
+        return true;
+      },
       [&](int i, uint2 v, uint32_t s) {
         const int64_t row = (int64_t)(i >> 3) * P;
         *reinterpret_cast<uint2*>(codes + row * PG_ROW + (i & 7) * 8) = v;
         scales[row * PG_SF + (i & 7)] = (uint8_t)s;
       });
-  if ((threadIdx.x & 31) == 0) (kv ? c.v_g : c.k_g)[page * P + slot] = g;
+  if (live && (threadIdx.x & 31) == 0) (kv ? c.v_g : c.k_g)[page * P + slot] = g;
 }
 
 template <int DT>
@@ -367,19 +375,30 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(fp4paged_cache 
   for (int r = threadIdx.x; r < n; r += PLAN_THREADS) c.lens[dst[r]] = w.start[r];
 }
 
-// Copies the planned pages, a (page, KV head) of one kind at a time per block.
+// Copies the planned pages.  A page's codes of all heads are contiguous, as are its scales and its g; a block takes a
+// quarter of a page's codes and scales of one kind at a time, four 16-byte loads in flight a thread.
+__device__ __forceinline__ void copy16(uint4* to, const uint4* from, int n) {
+  int j = threadIdx.x;
+  for (; j + 768 < n; j += 1024) {
+    uint4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = from[j + 256 * i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[j + 256 * i] = v[i];
+  }
+  for (; j < n; j += 256) to[j] = from[j];
+}
 __global__ void __launch_bounds__(256) fork_copy_kernel(fp4paged_cache c) {
   const Work w = work_of(c);
-  const int H = c.num_kv_heads, P = c.page_size, total = w.total[0];
-  for (int64_t i = blockIdx.x; i < (int64_t)total * 2 * H; i += gridDim.x) {
-    const int n = (int)(i / (2 * H)), h = (int)(i % (2 * H)) >> 1, kv = (int)i & 1;
-    const int64_t p0 = w.from[n], p1 = w.ids[n];
-    uint4* codes = reinterpret_cast<uint4*>(kv ? c.v_codes : c.k_codes);
-    uint4* scales = reinterpret_cast<uint4*>(kv ? c.v_scales : c.k_scales);
-    const int64_t a0 = (p0 * H + h) * P, a1 = (p1 * H + h) * P;
-    for (int j = threadIdx.x; j < 4 * P; j += 256) codes[a1 * 4 + j] = codes[a0 * 4 + j];
-    for (int j = threadIdx.x; j < P / 2; j += 256) scales[a1 / 2 + j] = scales[a0 / 2 + j];
-    if (h == 0) {
+  const int P = c.page_size, total = w.total[0], quarter = c.num_kv_heads * P;  // 16-byte units of a quarter's codes
+  for (int i = blockIdx.x; i < total * 8; i += gridDim.x) {
+    const int64_t p0 = w.from[i >> 3], p1 = w.ids[i >> 3];
+    const int kv = i & 1, q = (i >> 1) & 3;
+    uint4 *codes = reinterpret_cast<uint4*>(kv ? c.v_codes : c.k_codes) + (int64_t)q * quarter,
+          *scales = reinterpret_cast<uint4*>(kv ? c.v_scales : c.k_scales) + (int64_t)q * (quarter / 8);
+    copy16(codes + p1 * quarter * 4, codes + p0 * quarter * 4, quarter);
+    copy16(scales + p1 * (quarter / 2), scales + p0 * (quarter / 2), quarter / 8);
+    if (q == 0) {
       float* g = kv ? c.v_g : c.k_g;
       for (int j = threadIdx.x; j < P; j += 256) g[p1 * P + j] = g[p0 * P + j];
     }
@@ -387,34 +406,47 @@ __global__ void __launch_bounds__(256) fork_copy_kernel(fp4paged_cache c) {
 }
 
 // ------------------------------------------------------------------ gather
-// A thread per block of 16 channels: 8 code bytes and a scale byte in, 16 values out.
+// A thread per block of 16 channels of GT tokens, 32 apart: 8 code bytes, a scale byte and g in, 16 values out.  A
+// token's data is three trips to memory away (length, page, bytes), so the tokens' trips are made together (46 us for
+// 3 x 8192 tokens with one token a thread).
+constexpr int GT = 4;
 template <int DT>
 __global__ void __launch_bounds__(256) gather_kernel(fp4paged_cache c, void* k_out, void* v_out, const int32_t* seqs,
                                                      int T) {
   using E = typename In<DT>::T;
   const int H = c.num_kv_heads, P = c.page_size, bh = blockIdx.y, b = bh / H, h = bh % H, kv = blockIdx.z;
-  const int t = blockIdx.x * 32 + (threadIdx.x >> 3), j = threadIdx.x & 7;
-  if (t >= T) return;
-  const int s = pg_seq(c, seqs, b);
-  float y[16];
+  const int t0 = blockIdx.x * 32 * GT + (threadIdx.x >> 3), j = threadIdx.x & 7;
+  const int s = pg_seq(c, seqs, b), len = s < 0 ? 0 : min(c.lens[s], T);
+  const uint8_t *codes = kv ? c.v_codes : c.k_codes, *scales = kv ? c.v_scales : c.k_scales;
+  const float* gs = kv ? c.v_g : c.k_g;
+  int64_t page[GT];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) y[i] = 0.0f;
-  if (s >= 0 && t < c.lens[s]) {
-    const int64_t page = c.page_table[(int64_t)s * c.max_pages + t / P];
-    const int64_t row = (page * H + h) * P + t % P;
-    const uint2 w = *reinterpret_cast<const uint2*>((kv ? c.v_codes : c.k_codes) + row * PG_ROW + j * 8);
-    const float sc = e4m3_to_f32((kv ? c.v_scales : c.k_scales)[row * PG_SF + j]);
-    const float g = (kv ? c.v_g : c.k_g)[page * P + t % P];
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      y[i] = __fmul_rn(__fmul_rn(e2m1_value(((i < 8 ? w.x : w.y) >> (4 * (i & 7))) & 15u), sc), g);
+  for (int i = 0; i < GT; ++i) {
+    const int t = t0 + 32 * i;
+    page[i] = t < len ? c.page_table[(int64_t)s * c.max_pages + t / P] : -1;
   }
-  E* out = static_cast<E*>(kv ? v_out : k_out) + ((int64_t)bh * T + t) * PG_D + j * 16;
-  uint4 raw[sizeof(E)];
+  uint2 w[GT];
+  float sc[GT], g[GT];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) store_out<DT>(raw, i, y[i]);
+  for (int i = 0; i < GT; ++i) {
+    const int slot = (t0 + 32 * i) % P;
+    const int64_t row = (page[i] * H + h) * P + slot;
+    w[i] = page[i] >= 0 ? __ldg(reinterpret_cast<const uint2*>(codes + row * PG_ROW) + j) : make_uint2(0u, 0u);
+    sc[i] = page[i] >= 0 ? e4m3_to_f32(__ldg(scales + row * PG_SF + j)) : 0.0f;
+    g[i] = page[i] >= 0 ? __ldg(gs + page[i] * P + slot) : 0.0f;
+  }
 #pragma unroll
-  for (int i = 0; i < (int)sizeof(E); ++i) reinterpret_cast<uint4*>(out)[i] = raw[i];
+  for (int i = 0; i < GT; ++i) {
+    const int t = t0 + 32 * i;
+    if (t >= T) break;
+    uint4 raw[sizeof(E)];
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      store_out<DT>(raw, e, __fmul_rn(__fmul_rn(e2m1_value(((e < 8 ? w[i].x : w[i].y) >> (4 * (e & 7))) & 15u), sc[i]), g[i]));
+    uint4* out = reinterpret_cast<uint4*>(static_cast<E*>(kv ? v_out : k_out) + ((int64_t)bh * T + t) * PG_D + j * 16);
+#pragma unroll
+    for (int e = 0; e < (int)sizeof(E); ++e) out[e] = raw[e];
+  }
 }
 
 int check_cache(const fp4paged_cache* c) {
@@ -429,7 +461,7 @@ int check_cache(const fp4paged_cache* c) {
   if (c->head_dim != PG_D) return set_error(FP4ATTN_ERR_UNSUPPORTED, "head_dim must be %d", PG_D);
   if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128)
     return set_error(FP4ATTN_ERR_ARG, "page_size must be 16, 32, 64 or 128");
-  if (c->num_pages <= 0 || c->num_kv_heads <= 0 || c->num_kv_heads > 1024 || c->max_seqs <= 0 || c->max_pages <= 0)
+  if (c->num_pages <= 0 || c->num_pages > 1 << 27 || c->num_kv_heads <= 0 || c->num_kv_heads > 1024 || c->max_seqs <= 0 || c->max_pages <= 0)
     return set_error(FP4ATTN_ERR_ARG, "bad cache shape");
   // positions, and the sum of the pages that one call can ask for, are 32-bit
   if ((int64_t)c->max_pages * c->page_size > INT32_MAX || (int64_t)c->max_seqs * c->max_pages > INT32_MAX)
@@ -533,7 +565,7 @@ extern "C" int fp4paged_gather(const fp4paged_cache* cache, void* k_out, void* v
   if (!k_out || !v_out) return set_error(FP4ATTN_ERR_ARG, "k_out or v_out is null");
   if (((uintptr_t)k_out | (uintptr_t)v_out) % 16) return set_error(FP4ATTN_ERR_ARG, "outputs must be 16-byte aligned");
   if ((int64_t)B * cache->num_kv_heads > 65535) return set_error(FP4ATTN_ERR_ARG, "more than 65535 (row, head) pairs");
-  const dim3 grid((unsigned)((T + 31) / 32), (unsigned)(B * cache->num_kv_heads), 2);
+  const dim3 grid((unsigned)((T + 32 * GT - 1) / (32 * GT)), (unsigned)(B * cache->num_kv_heads), 2);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (out_dtype) {
     case FP4_DT_F32: gather_kernel<FP4_DT_F32><<<grid, 256, 0, st>>>(*cache, k_out, v_out, seqs, T); break;

@@ -57,7 +57,7 @@ def _int32(name: str, t: torch.Tensor | None, shape: tuple, device) -> int | Non
     """Address of an optional int32 device tensor of a call (None: NULL)."""
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.device != device or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.dtype != torch.int32 or t.device != device or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape} on {device}")
     return t.data_ptr()
 
@@ -93,18 +93,30 @@ class PagedNVFP4Cache:
         self.device = self.lens.device
         tensors = (self.k_codes, self.k_scales, self.k_g, self.v_codes, self.v_scales, self.v_g, self.page_table,
                    self.lens, self.refs, self.status, self._work)
+        self._index = self.device.index
+        self._work_bytes = {}  # workspace sizes of tree_attention by shape
+        self._spaces = []      # workspaces, the last one in use: older ones stay, as captured graphs may hold them
         self._struct = _Struct(*(t.data_ptr() for t in tensors), num_pages, page_size, num_kv_heads, head_dim,
                                max_seqs, max_pages_per_seq)
         self._ref = ctypes.addressof(self._struct)
 
     # ------------------------------------------------------------ helpers
     def _call(self, name: str, *args) -> None:
-        _lib.call(name, self._ref, *args, torch.cuda.current_stream(self.device).cuda_stream)
+        _lib.call(name, self._ref, *args, _lib.raw_stream(self._index))
+
+    def _workspace(self, B: int, Hq: int, N: int) -> torch.Tensor:
+        need = self._work_bytes.get((B, Hq, N))
+        if need is None:
+            need = self._work_bytes[B, Hq, N] = _lib.load().fp4paged_attention_workspace_size(B, Hq, self.num_kv_heads, N)
+        if not self._spaces or self._spaces[-1].numel() < need:
+            grown = max(need, 2 * self._spaces[-1].numel()) if self._spaces else need
+            self._spaces.append(torch.empty(grown, dtype=torch.uint8, device=self.device))
+        return self._spaces[-1]
 
     def _rows(self, seqs: torch.Tensor | None, B: int) -> int | None:
         if B > self.max_seqs:
             raise ValueError(f"{B} rows, the cache has {self.max_seqs} sequences")
-        return _int32("seqs", seqs, (B,), self.device)
+        return None if seqs is None else _int32("seqs", seqs, (B,), self.device)
 
     def check(self) -> None:
         """Wait for the GPU and raise if a call since the last check could not be carried out."""
@@ -118,21 +130,23 @@ class PagedNVFP4Cache:
                counts: torch.Tensor | None = None) -> None:
         """Quantize T new tokens per row, k and v [B, H, T, D] (post-RoPE K), and store them behind sequence
         seqs[b] (default: b); counts [B] int32: only the first counts[b] tokens of row b."""
-        _lib.require_cuda(k, v)
-        if k.dim() != 4 or k.shape != v.shape or k.shape[1] != self.num_kv_heads or k.shape[3] != self.head_dim:
+        shape, device = k.shape, self.device
+        if k.device != device or v.device != device:
+            _lib.require_cuda(k, v)
+            raise ValueError(f"k and v must be on {device}")
+        if len(shape) != 4 or shape != v.shape or shape[1] != self.num_kv_heads or shape[3] != self.head_dim:
             raise ValueError(f"k and v must be [B, {self.num_kv_heads}, T, {self.head_dim}]")
-        if k.device != self.device or v.device != self.device:
-            raise ValueError(f"k and v must be on {self.device}")
-        if k.dtype != v.dtype or k.dtype not in _lib.DTYPE_CODE:
+        code = _lib.DTYPE_CODE.get(k.dtype)
+        if code is None or k.dtype != v.dtype:
             raise ValueError("k and v must both be float32, bfloat16 or float16")
-        B, _, T, _ = k.shape
+        B, _, T, _ = shape
         if k.stride(3) != 1:
             k = k.contiguous()
         if v.stride(3) != 1:
             v = v.contiguous()
-        self._call("fp4paged_append", k.data_ptr(), v.data_ptr(), _lib.DTYPE_CODE[k.dtype], B, T, k.stride(0),
-                   k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2), self._rows(seqs, B),
-                   _int32("counts", counts, (B,), self.device))
+        ks, vs = k.stride(), v.stride()
+        self._call("fp4paged_append", k.data_ptr(), v.data_ptr(), code, B, T, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+                   self._rows(seqs, B), None if counts is None else _int32("counts", counts, (B,), device))
 
     def truncate(self, lens: torch.Tensor, seqs: torch.Tensor | None = None) -> None:
         """Row b keeps its first lens[b] tokens (int32 [B]) if it has more; pages nobody holds become free."""
@@ -174,8 +188,8 @@ class PagedNVFP4Cache:
             raise ValueError("T must not be negative")
         B = seqs.shape[0] if seqs is not None else self.max_seqs if B is None else B
         rows = self._rows(seqs, B)
-        kv = torch.empty(2, B, self.num_kv_heads, T, self.head_dim, dtype=dtype, device=self.device)
-        k, v = kv.unbind(0)
+        shape = (B, self.num_kv_heads, T, self.head_dim)
+        k, v = torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device)
         self._call("fp4paged_gather", k.data_ptr(), v.data_ptr(), _lib.DTYPE_CODE[dtype], rows, B, T)
         return k, v
 
@@ -211,40 +225,47 @@ def tree_attention(q: torch.Tensor, cache: PagedNVFP4Cache, mask: torch.Tensor |
     quantized: blocks of P would run over sibling nodes, so that a token's
     output would depend on what else was drafted.  The output has q's dtype
     unless out or out_dtype says otherwise.
+
+    workspace: a device buffer of fp4paged_attention_workspace_size bytes,
+    256-byte aligned (default: one that the cache keeps).
     """
-    _lib.require_cuda(q)
+    device = q.device
+    if device != cache.device:
+        _lib.require_cuda(q)
+        raise ValueError(f"q must be on {cache.device}")
     if q.dim() != 4:
         raise ValueError("q must be [B, Hq, N, D]")
     B, Hq, N, D = q.shape
     if D != cache.head_dim or Hq % cache.num_kv_heads or Hq == 0:
         raise ValueError(f"q [B, Hq, N, {cache.head_dim}] needs Hq a multiple of {cache.num_kv_heads}")
-    if q.device != cache.device:
-        raise ValueError(f"q must be on {cache.device}")
-    if q.dtype not in _lib.DTYPE_CODE:
+    in_code = _lib.DTYPE_CODE.get(q.dtype)
+    if in_code is None:
         raise ValueError("q must be float32, bfloat16 or float16")
-    if q.stride(3) != 1:
+    sB, sH, sN, sD = q.stride()
+    if sD != 1:
         q = q.contiguous()
+        sB, sH, sN, _ = q.stride()
     if out_dtype is None:
         out_dtype = q.dtype if out is None else out.dtype
-    if out_dtype not in _lib.DTYPE_CODE:
+    out_code = _lib.DTYPE_CODE.get(out_dtype)
+    if out_code is None:
         raise ValueError("the output must be float32, bfloat16 or float16")
     if out is None:
-        out = torch.empty(B, N, Hq, D, dtype=out_dtype, device=q.device)
-    elif out.shape != (B, N, Hq, D) or out.dtype != out_dtype or not out.is_contiguous() or out.device != q.device:
-        raise ValueError(f"out must be a contiguous {out_dtype} [B, N, Hq, D] tensor on {q.device}")
+        out = torch.empty((B, N, Hq, D), dtype=out_dtype, device=device)
+    elif out.shape != (B, N, Hq, D) or out.dtype != out_dtype or not out.is_contiguous() or out.device != device:
+        raise ValueError(f"out must be a contiguous {out_dtype} [B, N, Hq, D] tensor on {device}")
     mp, mB, mI, mJ = None, 0, 0, 0
     if mask is not None:
-        if mask.dtype != torch.bool or mask.device != q.device or mask.shape not in ((N, N), (B, N, N)):
-            raise ValueError(f"mask must be bool [N, N] or [B, N, N] on {q.device}")
+        if mask.dtype != torch.bool or mask.device != device or mask.shape not in ((N, N), (B, N, N)):
+            raise ValueError(f"mask must be bool [N, N] or [B, N, N] on {device}")
         mp, mI, mJ = mask.data_ptr(), mask.stride(-2), mask.stride(-1)
         mB = mask.stride(0) if mask.dim() == 3 else 0
     if B == 0 or N == 0:
         return out
-    need = _lib.load().fp4paged_attention_workspace_size(B, Hq, cache.num_kv_heads, N)
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    cache._call("fp4paged_attention", q.data_ptr(), _lib.DTYPE_CODE[q.dtype], B, Hq, N, q.stride(0), q.stride(1),
-                q.stride(2), mp, mB, mI, mJ, _int32("counts", counts, (B,), q.device), cache._rows(seqs, B),
-                D ** -0.5 if scaling is None else float(scaling), out.data_ptr(), _lib.DTYPE_CODE[out_dtype],
-                workspace.data_ptr(), workspace.numel() * workspace.element_size())
+        workspace = cache._workspace(B, Hq, N)
+    cache._call("fp4paged_attention", q.data_ptr(), in_code, B, Hq, N, sB, sH, sN, mp, mB, mI, mJ,
+                None if counts is None else _int32("counts", counts, (B,), device), cache._rows(seqs, B),
+                D ** -0.5 if scaling is None else float(scaling), out.data_ptr(), out_code, workspace.data_ptr(),
+                workspace.numel() * workspace.element_size())
     return out

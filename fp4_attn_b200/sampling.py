@@ -20,9 +20,7 @@ def _per_row(name: str, v, R: int, dtype: torch.dtype, device, off) -> torch.Ten
         if v.dtype != dtype or v.device != device or v.numel() != R or not v.is_contiguous():
             raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor of {R} values on {device}")
         return v
-    if v is None or v == off:
-        return None
-    return torch.full((R,), v, dtype=dtype, device=device)
+    return None if v is None or v == off else torch.full((R,), v, dtype=dtype, device=device)
 
 
 def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
@@ -45,21 +43,28 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     Probabilities are summed as whole multiples of 2^-34 of the row's largest, so
     the result does not depend on the order of the sums.
     """
-    _lib.require_cuda(logits, u)
-    if logits.dim() < 1 or logits.shape[-1] < 1:
+    dev, shape = logits.device, logits.shape
+    if dev.type != "cuda" or u.device != dev:
+        _lib.require_cuda(logits, u)
+        raise ValueError(f"u must be on {dev}")
+    if len(shape) < 1 or shape[-1] < 1:
         raise ValueError("logits must be [..., V] with V >= 1")
-    if logits.dtype not in _lib.DTYPE_CODE:
+    code = _lib.DTYPE_CODE.get(logits.dtype)
+    if code is None:
         raise ValueError("logits must be float32, bfloat16 or float16")
-    lead, V = logits.shape[:-1], logits.shape[-1]
+    lead, V = shape[:-1], shape[-1]
     if V > MAX_VOCAB:
         raise NotImplementedError(f"{V} logits in a row: the kernel takes up to {MAX_VOCAB}")
-    if u.shape != lead or u.dtype != torch.float32 or u.device != logits.device:
-        raise ValueError(f"u must be fp32 of shape {tuple(lead)} on {logits.device}")
-    dev = logits.device
-    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
-    if x.stride(1) != 1 and V > 1:
+    if u.shape != lead or u.dtype != torch.float32:
+        raise ValueError(f"u must be fp32 of shape {tuple(lead)}")
+    x = logits if len(shape) == 2 else logits.reshape(-1, V)
+    ld, step = x.stride()
+    if step != 1 and V > 1:
         x = x.contiguous()
+        ld = V
     R = x.shape[0]
+    if not u.is_contiguous():
+        u = u.contiguous()
     tokens = torch.empty(lead, dtype=torch.int64, device=dev)
     logprobs = torch.empty(lead, dtype=torch.float32, device=dev)
     if R == 0:
@@ -68,9 +73,9 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     k = _per_row("top_k", top_k, R, torch.int32, dev, 0)
     p = _per_row("top_p", top_p, R, torch.float32, dev, 1.0)
     m = _per_row("min_p", min_p, R, torch.float32, dev, 0.0)
-    _lib.call("fp4_sample", x.data_ptr(), _lib.DTYPE_CODE[x.dtype], R, V, x.stride(0), u.contiguous().data_ptr(),
-              _lib.ptr(t), _lib.ptr(k), _lib.ptr(p), _lib.ptr(m), tokens.data_ptr(), logprobs.data_ptr(),
-              _lib.stream_of(x))
+    ptr = _lib.ptr
+    _lib.call("fp4_sample", x.data_ptr(), code, R, V, ld, u.data_ptr(), ptr(t), ptr(k), ptr(p), ptr(m),
+              tokens.data_ptr(), logprobs.data_ptr(), _lib.raw_stream(dev.index))
     return tokens, logprobs
 
 
