@@ -58,20 +58,60 @@ __device__ __forceinline__ float pg_global(float m, float& r) {
   return bad ? __int_as_float(0x7fc00000) : g;
 }
 
-// A block under 1/g = r (0 in a token of zeros or NaN): eight code bytes and the E4M3 scale byte.
+// Packed fp32 pairs, each rounded like the scalar operation.
+__device__ __forceinline__ uint64_t pg_pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t pg_mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t pg_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// Eight floats, in pairs, to eight E2M1 codes (the first in the low nibble).
+__device__ __forceinline__ uint32_t pg_codes(const uint64_t (&z)[4]) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t.reg .f32 l, h;\n\t"
+      "mov.b64 {l, h}, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b0, h, l;\n\t"
+      "mov.b64 {l, h}, %2;\n\tcvt.rn.satfinite.e2m1x2.f32 b1, h, l;\n\t"
+      "mov.b64 {l, h}, %3;\n\tcvt.rn.satfinite.e2m1x2.f32 b2, h, l;\n\t"
+      "mov.b64 {l, h}, %4;\n\tcvt.rn.satfinite.e2m1x2.f32 b3, h, l;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(r)
+      : "l"(z[0]), "l"(z[1]), "l"(z[2]), "l"(z[3]));
+  return r;
+}
+
+// A block whose largest |x| is m, under 1/g = r (0 in a token of zeros or NaN): eight code bytes and the E4M3 scale
+// byte.  The largest |x r| is that of m: rounding keeps order.
 template <typename Blk>
-__device__ __forceinline__ uint32_t pg_block(const Blk& x, float r, uint2& codes) {
-  float y[16], m = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) y[i] = r == 0.0f ? 0.0f : __fmul_rn(x[i], r), m = fmaxf(m, fabsf(y[i]));
-  const uint32_t s8 = e4m3_satfinite(__fmul_rn(m, recip6<FP4_ARITH_F32>()));
+__device__ __forceinline__ uint32_t pg_block(const Blk& x, float m, float r, uint2& codes) {
+  codes = make_uint2(0u, 0u);
+  if (r == 0.0f) return 0u;  // the same for the whole token
+  const uint32_t s8 = e4m3_satfinite(__fmul_rn(__fmul_rn(m, r), recip6<FP4_ARITH_F32>()));
   const float s = e4m3_to_f32((uint8_t)s8), rs = s == 0.0f ? 0.0f : __frcp_rn(s);
-  uint32_t w[2] = {0u, 0u};
+  const uint64_t r2 = pg_pair(r, r), rs2 = pg_pair(rs, rs), zero = pg_pair(0.0f, 0.0f);
+  uint64_t z[2][4];
 #pragma unroll
-  for (int i = 0; i < 16; i += 2)  // + 0: a zero's code has no sign
-    w[i >> 3] |= e2m1x2(__fmul_rn(y[i], rs) + 0.0f, __fmul_rn(y[i + 1], rs) + 0.0f) << (4 * (i & 7));
-  codes = make_uint2(w[0], w[1]);
+  for (int i = 0; i < 8; ++i)  // + 0: a zero's code has no sign
+    z[i >> 2][i & 3] = pg_add2(pg_mul2(pg_mul2(pg_pair(x[2 * i], x[2 * i + 1]), r2), rs2), zero);
+  codes = make_uint2(pg_codes(z[0]), pg_codes(z[1]));
   return s8;
+}
+
+// Four E2M1 code pairs (the bytes of w, lowest first) as fp16 pairs.
+__device__ __forceinline__ void e2m1x8_f16(uint32_t w, uint32_t* o) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\tmov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\tcvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3])
+      : "r"(w));
 }
 
 // A warp quantizes one token of H heads: lane l takes blocks l, l + 32, ...; at(block) is where the block's
@@ -88,9 +128,10 @@ __device__ __forceinline__ float pg_quantize_token(int nblk, At at, Where where,
     for (int i = 0; i < NB; ++i)
       if (lane + 32 * i < nblk) x[i].load(at(lane + 32 * i));
     if (!where()) return 0.0f;
+    float top[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i)
-      if (lane + 32 * i < nblk) m = nanmax(m, x[i].absmax());
+      if (lane + 32 * i < nblk) top[i] = x[i].absmax(), m = nanmax(m, top[i]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = nanmax(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float g = pg_global(m, r);
@@ -98,7 +139,7 @@ __device__ __forceinline__ float pg_quantize_token(int nblk, At at, Where where,
     for (int i = 0; i < NB; ++i)
       if (lane + 32 * i < nblk) {
         uint2 c;
-        const uint32_t s = pg_block(x[i], r, c);
+        const uint32_t s = pg_block(x[i], top[i], r, c);
         put(lane + 32 * i, c, s);
       }
     return g;
@@ -112,7 +153,7 @@ __device__ __forceinline__ float pg_quantize_token(int nblk, At at, Where where,
     for (int i = lane; i < nblk; i += 32) {
       x.load(at(i));
       uint2 c;
-      const uint32_t s = pg_block(x, r, c);
+      const uint32_t s = pg_block(x, x.absmax(), r, c);
       put(i, c, s);
     }
     return g;

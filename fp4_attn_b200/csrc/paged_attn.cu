@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(PREP_THREADS) paged_prep_kernel(AttnArgs a, Pr
     const float g = pg_global(m, r);
     auto put = [&](int i, const Block16<DT, VEC>& b) {
       uint2 c;
-      const uint32_t s = pg_block(b, r, c);
+      const uint32_t s = pg_block(b, b.absmax(), r, c);
       const int64_t row = row_of(i >> 3);
       *reinterpret_cast<uint2*>(const_cast<uint8_t*>(a.q_codes) + row * PG_ROW + (i & 7) * 8) = c;
       const_cast<uint8_t*>(a.q_scales)[row * PG_SF + (i & 7)] = (uint8_t)s;
@@ -395,15 +395,6 @@ __device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t two_bytes) {
   asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(r) : "r"(two_bytes));
   return r;
 }
-// Four E2M1 code pairs (the bytes of w, lowest first) as fp16 pairs.
-__device__ __forceinline__ void e2m1x8_f16(uint32_t w, uint32_t* o) {
-  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\tmov.b32 {b0, b1, b2, b3}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\tcvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
-      : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3])
-      : "r"(w));
-}
-
 __device__ __forceinline__ float rcp(float x) {
   float r;
   asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));

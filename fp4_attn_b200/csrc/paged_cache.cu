@@ -440,9 +440,17 @@ __global__ void __launch_bounds__(256) gather_kernel(fp4paged_cache c, void* k_o
     const int t = t0 + 32 * i;
     if (t >= T) break;
     uint4 raw[sizeof(E)];
+    uint32_t o[8];  // codes as fp16; times their scale they are exact
+    e2m1x8_f16(w[i].x, o), e2m1x8_f16(w[i].y, o + 4);
+    const __half2 s2 = __half2half2(__float2half_rn(sc[i]));
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
-      store_out<DT>(raw, e, __fmul_rn(__fmul_rn(e2m1_value(((e < 8 ? w[i].x : w[i].y) >> (4 * (e & 7))) & 15u), sc[i]), g[i]));
+    for (int e = 0; e < 8; ++e) {
+      const float2 v = __half22float2(__hmul2(*reinterpret_cast<const __half2*>(&o[e]), s2));
+      const float x0 = __fmul_rn(v.x, g[i]), x1 = __fmul_rn(v.y, g[i]);
+      if constexpr (DT == FP4_DT_F32) reinterpret_cast<float2*>(raw)[e] = make_float2(x0, x1);
+      else if constexpr (DT == FP4_DT_BF16) reinterpret_cast<__nv_bfloat162*>(raw)[e] = __floats2bfloat162_rn(x0, x1);
+      else reinterpret_cast<__half2*>(raw)[e] = __floats2half2_rn(x0, x1);
+    }
     uint4* out = reinterpret_cast<uint4*>(static_cast<E*>(kv ? v_out : k_out) + ((int64_t)bh * T + t) * PG_D + j * 16);
 #pragma unroll
     for (int e = 0; e < (int)sizeof(E); ++e) out[e] = raw[e];
