@@ -49,9 +49,9 @@ __device__ __forceinline__ uint32_t sp_key(float x) {
 
 __device__ __forceinline__ float logit_of(uint32_t q) { return __uint_as_float(q & 0x80000000u ? q & 0x7fffffffu : ~q); }
 
-constexpr int SP_THREADS = 512, SP_WARPS = SP_THREADS / 32;
 constexpr int SP_BINS = 512;    // of x's distance from the maximum
 constexpr int SP_LIST = 1024;   // logits of a bin that are ranked directly; more of them are searched bit by bit
+constexpr int SP_SHORT = 256;   // that many, and all bins down to one are ranked together
 constexpr int SP_RANKS = 16;    // CTAs of a cluster
 constexpr int SP_LIMB = 17;     // a weight as two parts of 17 bits,
 constexpr int SP_HELD = 32767;  // of which this many add up within 32 bits: logits that a CTA holds
@@ -72,39 +72,36 @@ struct alignas(16) SampleShared {  // (16-byte loads follow it)
   uint32_t mine_key[SP_LIST];  // this CTA's part of the list
   int mine_index[SP_LIST];
   int listed, found, last;
-  u64 found_before, last_mass;
+  u64 last_mass;
   Cut cut;
   float rank_max[SP_RANKS], rank_min[SP_RANKS];
   u64 rank_sum[4][SP_RANKS];  // by turns; a slot is written anew only several barriers after it was read
   int rank_first[SP_RANKS];
-  u64 part[SP_WARPS], warp_sum[SP_WARPS];
-  int ipart[SP_WARPS];
-  float fpart[2][SP_WARPS];
+  u64 part[32], warp_sum[32];  // a value per warp
+  int ipart[32];
+  float fpart[2][32];
 };
 
-template <typename T>
+template <int NT, typename T>
 __device__ __forceinline__ T sp_block_sum(T v, T* part) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = part[threadIdx.x & (SP_WARPS - 1)];
+  v = part[threadIdx.x & ((NT / 32) - 1)];
 #pragma unroll
-  for (int o = SP_WARPS / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = (NT / 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
 // The first bin at which the running sum of v reaches `target`, and the sum before it; SP_BINS if it never does.
-template <typename T>
+template <int NT, typename T>
 __device__ __forceinline__ int sp_find_bin(SampleShared& sh, const T* v, double target) {
-  constexpr int PER = SP_BINS / SP_THREADS;
+  static_assert(SP_BINS <= NT, "a bin per thread");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  T own[PER];
-  u64 sum = 0;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) sum += own[i] = v[threadIdx.x * PER + i];
-  u64 inc = sum;
+  const u64 own = threadIdx.x < SP_BINS ? v[threadIdx.x] : 0;
+  u64 inc = own;
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) {
     const u64 u = __shfl_up_sync(0xffffffffu, inc, o);
@@ -114,21 +111,21 @@ __device__ __forceinline__ int sp_find_bin(SampleShared& sh, const T* v, double 
   if (lane == 31) sh.part[warp] = inc;
   if (threadIdx.x == 0) sh.found = SP_BINS;
   __syncthreads();
-  u64 at = inc - sum;
+  u64 at = inc - own;
 #pragma unroll
-  for (int i = 0; i < SP_WARPS; ++i) at += i < warp ? sh.part[i] : 0;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    if ((double)at < target && (double)(at + own[i]) >= target) sh.found = threadIdx.x * PER + i, sh.found_before = at;
-    at += own[i];
-  }
+  for (int i = 0; i < SP_BINS / 32; ++i) at += i < warp ? sh.part[i] : 0;
+  if ((double)at < target && (double)(at + own) >= target) sh.found = threadIdx.x;
   __syncthreads();
   return sh.found;
 }
 
-// STREAM: one CTA per row, which reads it anew each time; else a cluster's CTAs hold it.
+// STREAM: one CTA per row, which reads it anew each time (1024 threads, one CTA on an SM: the rows under way then fit
+// L2; with two they did not, and 512 rows of 131072 fp32 took 277 us); else a cluster's CTAs hold it.
+constexpr int SP_HELD_THREADS = 512, SP_STREAM_THREADS = 1024;
 template <int DT, bool STREAM>
-__global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a, int loads) {
+__global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, STREAM ? 1 : 2)
+    sample_kernel(SampleArgs a, int loads) {
+  constexpr int SP_THREADS = STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, SP_WARPS = SP_THREADS / 32;
   using T = typename In<DT>::T;
   constexpr int VEC = 16 / (int)sizeof(T);
   namespace cg = cooperative_groups;
@@ -266,7 +263,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a, int
   int turn = 0;
   // The cluster's sum of a number per thread.
   auto row_sum = [&](u64 v) -> u64 {
-    v = sp_block_sum(v, sh.part);
+    v = sp_block_sum<SP_THREADS>(v, sh.part);
     if (tid < C) peer(tid).rank_sum[turn & 3][rank] = v;
     barrier();
     u64 sum = 0;
@@ -361,7 +358,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a, int
         });
     first = __reduce_min_sync(0xffffffffu, first);
     if (lane == 0) sh.ipart[warp] = first;
-    z = sp_block_sum(z, sh.part);
+    z = sp_block_sum<SP_THREADS>(z, sh.part);
     if (tid < C) {
       int m = INT32_MAX;
 #pragma unroll
@@ -429,33 +426,39 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a, int
     // the bin where the count, or the mass, reaches the target, in this band or one further away; SP_BINS: nowhere
     auto locate = [&](bool by_mass, double target) -> int {
       for (;;) {
-        const int b = by_mass ? sp_find_bin(sh, sh.mass, target - (double)base_w) : sp_find_bin(sh, sh.total, target - (double)base_n);
+        const int b = by_mass ? sp_find_bin<SP_THREADS>(sh, sh.mass, target - (double)base_w) : sp_find_bin<SP_THREADS>(sh, sh.total, target - (double)base_n);
         if (b < SP_BINS || reach >= full) return b;
         u64 sn = 0, sw = 0;
         for (int i = tid; i < SP_BINS; i += SP_THREADS) sn += sh.total[i], sw += sh.mass[i];
-        base_n += sp_block_sum(sn, sh.part), base_w += sp_block_sum(sw, sh.part);
+        base_n += sp_block_sum<SP_THREADS>(sn, sh.part), base_w += sp_block_sum<SP_THREADS>(sw, sh.part);
         if (!(merged = merged && band(reach, fminf(full, reach * 1.3f)))) return SP_BINS;
       }
     };
-    int listed_bin = -1, n = 0;
+    int listed_bin = -1, listed_from = 0, n = 0;  // the bins that are listed
     u64 above_n = 0, above_w = 0;
     int at_n[SP_LIST / SP_THREADS];
     u64 at_w[SP_LIST / SP_THREADS];
-    // the bin's logits, and how many and how much goes before each of this thread's
+    // The logits of a bin -- or, where they are few, of all bins of the band up to it: top_p then finds its cut among
+    // them too -- and how many and how much goes before each of this thread's.
     auto list = [&](int bin) {
       if (listed_bin >= 0) {
         barrier();  // (the last list has been read)
         if (tid == 0) sh.listed = 0;
         barrier();
       }
-      listed_bin = bin;
+      u64 sn = 0, sw = 0;
+      for (int i = tid; i < bin; i += SP_THREADS) sn += sh.total[i], sw += sh.mass[i];
+      sn = sp_block_sum<SP_THREADS>(sn, sh.part);
+      const bool all = by_k && by_p && sn + sh.total[bin] <= SP_SHORT;
+      above_n = base_n + (all ? 0 : sn), above_w = base_w + (all ? 0 : sp_block_sum<SP_THREADS>(sw, sh.part));
+      listed_bin = bin, listed_from = all ? 0 : bin;
       // (a range that surely has the bin, to pass over the others quickly)
       const float wide = fabsf(mx) * 2.4e-7f, at0 = mx - fmaxf(from, 0.0f);
-      const float hi = bin ? at0 - (float)(bin - 1) / per + wide : INFINITY;
+      const float hi = listed_from ? at0 - (float)(listed_from - 1) / per + wide : INFINITY;
       const float lo = per > 0.0f ? at0 - (float)(bin + 2) / per - wide : -INFINITY;
       each([&](float v) { return v >= lo && v <= hi; },
            [&](float v, int index) {
-             if (in_band(v) && bin_of(v) == bin) {
+             if (in_band(v) && bin_of(v) >= listed_from && bin_of(v) <= bin) {
                const int at = atomicAdd(&sh.listed, 1);
                if (at < SP_LIST) sh.mine_key[at] = sp_key(v), sh.mine_index[at] = index;
              }
@@ -474,9 +477,6 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a, int
         sh.list[e] = (u64)q << 32 | (uint32_t)~peer(c).mine_index[i], sh.list_w[e] = weight(logit_of(q));
       }
       __syncthreads();
-      u64 sn = 0, sw = 0;
-      for (int i = tid; i < bin; i += SP_THREADS) sn += sh.total[i], sw += sh.mass[i];
-      above_n = base_n + sp_block_sum(sn, sh.part), above_w = base_w + sp_block_sum(sw, sh.part);
 #pragma unroll
       for (int t = 0; t < SP_LIST / SP_THREADS; ++t) {
         const int e = tid + t * SP_THREADS;
@@ -524,14 +524,14 @@ __global__ void __launch_bounds__(SP_THREADS, 2) sample_kernel(SampleArgs a, int
       const double target = p_target(mass);
       if ((double)base_w >= target) {  // top_k went past the band that has it
         base_n = base_w = 0;
-        listed_bin = SP_BINS;
+        listed_bin = listed_from = SP_BINS;
         merged = band(-1.0f, near);
       }
       const int b = merged ? locate(true, target) : SP_BINS;
       if (b == SP_BINS || sh.total[b] > SP_LIST) {
         search = true;
       } else {
-        if (b != listed_bin) list(b);
+        if (b > listed_bin || b < listed_from) list(b);
         // (what top_k dropped has all of `mass` before it, more than the target)
         settle([&](int t) { return (double)(above_w + at_w[t]) < target; });
       }
@@ -644,12 +644,13 @@ int launch_sample(const SampleArgs& a, cudaStream_t st) {
   if (stream) C = 1;
   else
     while (C < 8 && (int64_t)a.R * C * 2 <= 296 && C * 4096 < n) C *= 2;
-  const int per_load = C * SP_THREADS * VEC, loads = (n + per_load - 1) / per_load;
-  const size_t smem = sizeof(SampleShared) + (stream ? 0 : (size_t)loads * SP_THREADS * 16);
+  const int threads = stream ? SP_STREAM_THREADS : SP_HELD_THREADS;
+  const int per_load = C * threads * VEC, loads = (n + per_load - 1) / per_load;
+  const size_t smem = sizeof(SampleShared) + (stream ? 0 : (size_t)loads * threads * 16);
   auto* fn = stream ? sample_kernel<DT, true> : sample_kernel<DT, false>;
   if (int e = set_smem_attr((const void*)fn, (int)sizeof(SampleShared) + 73728, true)) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(a.R * C)), cfg.blockDim = dim3(SP_THREADS);
+  cfg.gridDim = dim3((unsigned)(a.R * C)), cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem, cfg.stream = st;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeClusterDimension;
