@@ -12,7 +12,8 @@
 // Few rows: a cluster of CTAs reads a row once and holds it in shared memory; the
 // CTAs exchange their maxima, sums, histograms and the bin's logits over
 // distributed shared memory, and each draws the same conclusions from them.  Many rows: one
-// CTA per row goes over it several times, the later times mostly in L2.
+// CTA per row goes over it twice, the second time mostly in L2, and keeps the logits near the
+// maximum, which are what the rest needs, in shared memory.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -79,6 +80,7 @@ struct alignas(16) SampleShared {  // (16-byte loads follow it)
   int rank_first[SP_RANKS];
   u64 part[32], warp_sum[32];  // a value per warp
   int ipart[32];
+  int near_n[32];  // a streamed row's logits near the maximum, by warp
   float fpart[2][32];
 };
 
@@ -119,9 +121,10 @@ __device__ __forceinline__ int sp_find_bin(SampleShared& sh, const T* v, double 
   return sh.found;
 }
 
-// STREAM: one CTA per row, which reads it anew each time (1024 threads, one CTA on an SM: the rows under way then fit
+// STREAM: one CTA per row, which reads it anew for each pass (1024 threads, one CTA on an SM: the rows under way then fit
 // L2; with two they did not, and 512 rows of 131072 fp32 took 277 us); else a cluster's CTAs hold it.
 constexpr int SP_HELD_THREADS = 512, SP_STREAM_THREADS = 1024;
+constexpr int SP_NEAR = 640;  // logits of a band that a warp keeps (160 KB in all); more: the row is read again instead
 template <int DT, bool STREAM>
 __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, STREAM ? 1 : 2)
     sample_kernel(SampleArgs a, int loads) {
@@ -165,6 +168,9 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
   // and only few logits go further than a comparison.
   auto clean = [](float v) { return fminf(fmaxf(v, -INFINITY), SP_FAR); };
   auto value = [&](const uint4& raw, int i) { return In<DT>::f(reinterpret_cast<const T*>(&raw)[i]); };
+  u64* kept_near = reinterpret_cast<u64*>(held) + warp * SP_NEAR;  // (x, index), in no order
+  bool have_near = false;  // all down to near_reach below the maximum are there
+  float near_reach = 0.0f;
   auto index_of = [&](int j) { return pos0 + j * 32 * VEC - skip; };
   auto load = [&](int j) { return STREAM ? fetch(j) : mine[j * 32]; };
   // Calls see(x) for each of this thread's logits (not cleaned), and got(x, index) (cleaned) for those that it is true
@@ -205,6 +211,26 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
     }
   };
 
+  // each() over what is known to have all that see() is true for: the kept ones, if all of those are asked for
+  auto each_near = [&](bool enough, auto see, auto got) {
+    if (STREAM && enough && have_near) {
+      for (int e = lane; e < sh.near_n[warp]; e += 32) {
+        const u64 c = kept_near[e];
+        const float v = __uint_as_float((uint32_t)(c >> 32));
+        if (see(v)) got(v, (int)(uint32_t)c);
+      }
+    } else {
+      each(see, got);
+    }
+  };
+
+  auto keep_near = [&](float v, int index) {
+    if constexpr (STREAM) {
+      const int at = atomicAdd(&sh.near_n[warp], 1);
+      if (at < SP_NEAR) kept_near[at] = (u64)__float_as_uint(v) << 32 | (uint32_t)index;
+    }
+  };
+
   // --------------------------------------------------------- maximum, minimum
   if constexpr (!STREAM) {
 #pragma unroll 4
@@ -212,6 +238,7 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
   }
   for (int i = tid; i < SP_BINS; i += SP_THREADS) sh.count[i] = sh.lo[i] = sh.hi[i] = 0u;
   if (tid == 0) sh.listed = 0;
+  if (STREAM && lane == 0) sh.near_n[warp] = 0;
   float mx = -INFINITY, mn = INFINITY;  // mn: of those above -inf
   each(
       [&](float v) {
@@ -255,8 +282,9 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
   const double f = 1.4426950408889634 / (double)temp;
   const float f1 = (float)f, f2 = (float)(f - (double)f1);
   auto weight = [&](float v) -> u64 {
-    const float d = fminf(v, SP_FAR) - mx;
-    float e;  // (a NaN or an infinite d gives NaN or -inf, and so 0)
+    float e;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(e) : "f"(v), "f"(SP_FAR));  // (stays NaN)
+    const float d = e - mx;  // (a NaN or an infinite d gives NaN or -inf, and so 0)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaxf(fmaf(d, f1, d * f2), -150.0f)));
     return __float2ull_rn(e * SP_ONE);  // (2^34 in the exponent's argument would cost it four bits)
   };
@@ -328,10 +356,10 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
   };
 
   // ------------------------------- sum, first largest logit, first histogram
-  // of what can hold the thresholds: first the logits within 6 (or 6 T) of the maximum, which are few and mostly
+  // of what can hold the thresholds: first the logits within 7 (or 7 T) of the maximum, which are few and mostly
   // enough; a logit in the histogram costs as much as three that are only summed, a second histogram a pass over the row
   const float full = fminf(24.6f * temp, mx - mn);  // weights further away are 0
-  const float near = full <= 8.0f ? full : fminf(fmaxf(6.0f * temp, 6.0f), full);
+  const float near = full <= 8.0f ? full : fminf(fmaxf(7.0f * temp, 7.0f), full);
   float from = -1.0f, reach = near, per = reach > 0.0f ? (float)SP_BINS / reach : 0.0f;  // the band (from, reach] below mx
   auto in_band = [&](float v) { return mx - v > from && mx - v <= reach; };
   auto bin_of = [&](float v) { return max(0, min(SP_BINS - 1, (int)((mx - v - fmaxf(from, 0.0f)) * per))); };
@@ -346,7 +374,7 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
   int first = INT32_MAX;
   {
     // hits: what the histogram takes, or a greedy row's largest
-    const float low = greedy ? mx : by_k || by_p ? mx - reach : INFINITY;
+    const float low = greedy ? mx : by_k || by_p ? mx - reach - fabsf(mx) * 2.4e-7f : INFINITY;
     each(
         [&](float v) {
           z += weight(v);
@@ -354,8 +382,14 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
         },
         [&](float v, int index) {
           if (greedy) first = min(first, index);
-          else if (in_band(v)) add(v);
+          else if (in_band(v)) {
+            add(v);
+            keep_near(v, index);
+          }
         });
+    __syncwarp();
+    have_near = __syncthreads_and(STREAM && sh.near_n[warp] <= SP_NEAR && (by_k || by_p));
+    near_reach = reach;
     first = __reduce_min_sync(0xffffffffu, first);
     if (lane == 0) sh.ipart[warp] = first;
     z = sp_block_sum<SP_THREADS>(z, sh.part);
@@ -417,9 +451,16 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
       __syncthreads();
       const float upper = from < 0.0f ? INFINITY : mx - from + fabsf(mx) * 2.4e-7f, lower = mx - reach - fabsf(mx) * 2.4e-7f;
       each([&](float v) { return v >= lower && v <= upper; },
-           [&](float v, int) {
-             if (in_band(v)) add(v);
+           [&](float v, int index) {
+             if (!in_band(v)) return;
+             add(v);
+             if (have_near && reach > near_reach) keep_near(v, index);
            });
+      __syncwarp();
+      if (STREAM && have_near && reach > near_reach) {  // (bands follow one another)
+        have_near = __syncthreads_and(sh.near_n[warp] <= SP_NEAR);
+        near_reach = reach;
+      }
       barrier();
       return merge();
     };
@@ -431,7 +472,7 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
         u64 sn = 0, sw = 0;
         for (int i = tid; i < SP_BINS; i += SP_THREADS) sn += sh.total[i], sw += sh.mass[i];
         base_n += sp_block_sum<SP_THREADS>(sn, sh.part), base_w += sp_block_sum<SP_THREADS>(sw, sh.part);
-        if (!(merged = merged && band(reach, fminf(full, reach * 1.3f)))) return SP_BINS;
+        if (!(merged = merged && band(reach, fminf(full, reach * 1.15f)))) return SP_BINS;
       }
     };
     int listed_bin = -1, listed_from = 0, n = 0;  // the bins that are listed
@@ -456,7 +497,8 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
       const float wide = fabsf(mx) * 2.4e-7f, at0 = mx - fmaxf(from, 0.0f);
       const float hi = listed_from ? at0 - (float)(listed_from - 1) / per + wide : INFINITY;
       const float lo = per > 0.0f ? at0 - (float)(bin + 2) / per - wide : -INFINITY;
-      each([&](float v) { return v >= lo && v <= hi; },
+      each_near(
+           reach <= near_reach, [&](float v) { return v >= lo && v <= hi; },
            [&](float v, int index) {
              if (in_band(v) && bin_of(v) >= listed_from && bin_of(v) <= bin) {
                const int at = atomicAdd(&sh.listed, 1);
@@ -618,7 +660,7 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
         },
         [](float, int) {});
   } else {
-    each([&](float v) { return v >= edge; }, [&](float v, int index) { own += kept(v, index); });
+    each_near(mx - edge <= near_reach, [&](float v) { return v >= edge; }, [&](float v, int index) { own += kept(v, index); });
   }
   const Before s = row_scan(own);  // its barrier is behind the last access to another CTA's memory
   const u64 target = min((u64)floor((double)a.u[r] * (double)s.total), s.total - 1);
@@ -646,9 +688,9 @@ int launch_sample(const SampleArgs& a, cudaStream_t st) {
     while (C < 8 && (int64_t)a.R * C * 2 <= 296 && C * 4096 < n) C *= 2;
   const int threads = stream ? SP_STREAM_THREADS : SP_HELD_THREADS;
   const int per_load = C * threads * VEC, loads = (n + per_load - 1) / per_load;
-  const size_t smem = sizeof(SampleShared) + (stream ? 0 : (size_t)loads * threads * 16);
+  const size_t smem = sizeof(SampleShared) + (stream ? (size_t)32 * SP_NEAR * 8 : (size_t)loads * threads * 16);
   auto* fn = stream ? sample_kernel<DT, true> : sample_kernel<DT, false>;
-  if (int e = set_smem_attr((const void*)fn, (int)sizeof(SampleShared) + 73728, true)) return e;
+  if (int e = set_smem_attr((const void*)fn, (int)sizeof(SampleShared) + (stream ? 32 * SP_NEAR * 8 : 73728), true)) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.R * C)), cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem, cfg.stream = st;

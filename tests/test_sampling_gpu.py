@@ -139,6 +139,23 @@ def test_rows_that_are_not_finite():
         assert lp[4] == 0
 
 
+@pytest.mark.parametrize("rows", [3, 320])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_nan_in_masked_places(rows, dtype):
+    """Whole stretches of NaN, at the start among them, weigh nothing."""
+    V = 60001
+    x, u = logits(rows, V, dtype, seed=rows)
+    x[:, :20000] = float("nan")
+    x[:, 30000::7] = float("nan")
+    for kw in ({}, dict(m=0.05), dict(k=40, p=0.7), dict(T=0.0)):
+        u[0] = 0.0
+        tok, _ = run(x[:3], u[:3], **kw)
+        from fp4_attn_b200.sampling import sample
+        many = sample(x, u, temperature=kw.get("T", 1.0), top_k=kw.get("k", 0), top_p=kw.get("p", 1.0), min_p=kw.get("m", 0.0))
+        assert torch.equal(many[0][:3].cpu(), torch.as_tensor(tok).cpu())
+        assert (many[0] >= 20000).all() and torch.isfinite(x.gather(1, many[0][:, None])).all()
+
+
 def test_strides_shapes_and_streams():
     from fp4_attn_b200.sampling import sample
     x, u = logits(6, 777, torch.bfloat16, seed=3)
