@@ -20,6 +20,7 @@
 
 #include <algorithm>
 
+#include "attn_softmax.cuh"
 #include "common.cuh"
 #include "fp4attn.h"
 #include "status.h"
@@ -80,7 +81,6 @@ struct alignas(16) SampleShared {  // (16-byte loads follow it)
   int rank_first[SP_RANKS];
   u64 part[32], warp_sum[32];  // a value per warp
   int ipart[32];
-  int near_n[32];  // a streamed row's logits near the maximum, by warp
   float fpart[2][32];
 };
 
@@ -168,16 +168,17 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
   // and only few logits go further than a comparison.
   auto clean = [](float v) { return fminf(fmaxf(v, -INFINITY), SP_FAR); };
   auto value = [&](const uint4& raw, int i) { return In<DT>::f(reinterpret_cast<const T*>(&raw)[i]); };
-  u64* kept_near = reinterpret_cast<u64*>(held) + warp * SP_NEAR;  // (x, index), in no order
-  bool have_near = false;  // all down to near_reach below the maximum are there
+  u64* kept_near = reinterpret_cast<u64*>(held) + warp * SP_NEAR;  // (x or NaN, index), this warp's
+  int near_n = 0;
+  bool have_near = false;  // all warps have all down to near_reach below the maximum
   float near_reach = 0.0f;
   auto index_of = [&](int j) { return pos0 + j * 32 * VEC - skip; };
   auto load = [&](int j) { return STREAM ? fetch(j) : mine[j * 32]; };
-  // Calls see(x) for each of this thread's logits (not cleaned), and got(x, index) (cleaned) for those that it is true
-  // for.  The hits of up to 16 logits are gathered in a word first: got's code stands once, and the others cost little.
+  // Calls see(x, y), which answers with two bits, for each two of this thread's logits (not cleaned), and some(hits, j)
+  // with the bits of up to 16 of them, from load j on; all lanes of a warp call it together.
   constexpr int STEP = STREAM ? 16 / VEC : 8 / VEC;
   const bool inner = (rank * SP_WARPS + warp) * loads * 32 * VEC >= skip && (rank * SP_WARPS + warp + 1) * loads * 32 * VEC <= end;
-  auto each = [&](auto see, auto got) {
+  auto walk = [&](auto see, auto some) {
 #pragma unroll 1
     for (int j = 0; j < loads; j += STEP) {
       uint4 raw[STEP];
@@ -198,23 +199,31 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
       }
       uint32_t hits = 0u;
 #pragma unroll
-      for (int i = 0; i < STEP * VEC; ++i) hits |= (see(value(raw[i / VEC], i % VEC)) ? 1u : 0u) << i;
+      for (int i = 0; i < STEP * VEC; i += 2) hits |= see(value(raw[i / VEC], i % VEC), value(raw[i / VEC], i % VEC + 1)) << i;
+      some(hits, j);
+    }
+  };
+  auto place = [&](int j, int i) { return pos0 + (j + i / VEC) * 32 * VEC + i % VEC; };
+  auto real = [&](int j, int i) { return j + i / VEC < loads && place(j, i) >= skip && place(j, i) < end; };  // else a stand-in
+  // Calls got(x, index) (cleaned) for those that see(x) is true for.
+  auto each = [&](auto see, auto got) {
+    walk([&](float x, float y) { return (see(x) ? 1u : 0u) | (see(y) ? 2u : 0u); }, [&](uint32_t hits, int j) {
 #pragma unroll 1
       while (hits) {
         const int i = __ffs(hits) - 1;
         hits &= hits - 1;
-        const int at = pos0 + (j + i / VEC) * 32 * VEC + i % VEC;
-        if (j + i / VEC >= loads || at < skip || at >= end) continue;  // what stands in for no logit
-        const T v = STREAM ? __ldg(row + (at - skip)) : reinterpret_cast<const T*>(mine + (j + i / VEC) * 32)[i % VEC];
-        got(clean(In<DT>::f(v)), at - skip);
+        if (!real(j, i)) continue;
+        const int index = place(j, i) - skip;
+        const T v = STREAM ? __ldg(row + index) : reinterpret_cast<const T*>(mine + (j + i / VEC) * 32)[i % VEC];
+        got(clean(In<DT>::f(v)), index);
       }
-    }
+    });
   };
 
   // each() over what is known to have all that see() is true for: the kept ones, if all of those are asked for
   auto each_near = [&](bool enough, auto see, auto got) {
     if (STREAM && enough && have_near) {
-      for (int e = lane; e < sh.near_n[warp]; e += 32) {
+      for (int e = lane; e < near_n; e += 32) {
         const u64 c = kept_near[e];
         const float v = __uint_as_float((uint32_t)(c >> 32));
         if (see(v)) got(v, (int)(uint32_t)c);
@@ -224,11 +233,50 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
     }
   };
 
-  auto keep_near = [&](float v, int index) {
-    if constexpr (STREAM) {
-      const int at = atomicAdd(&sh.near_n[warp], 1);
-      if (at < SP_NEAR) kept_near[at] = (u64)__float_as_uint(v) << 32 | (uint32_t)index;
+  // A streamed row's hits are few, in some lanes: got(x, index) for them one by one would take longer than all else.
+  // Their indices go to the warp's list (behind those that are there), and got is called for 32 of them at a time; what
+  // it is false for counts no longer.  A list that is too long is given up, and each() takes its place.
+  auto take = [&](auto see, auto also, auto got) {
+    const int n0 = near_n;
+    walk([&](float x, float y) { also(x, y); return (see(x) ? 1u : 0u) | (see(y) ? 2u : 0u); },
+         [&](uint32_t hits, int j) {
+           if (!inner) {
+#pragma unroll 1
+             for (int i = 0; i < STEP * VEC; ++i)
+               if (!real(j, i)) hits &= ~(1u << i);
+           }
+           unsigned any;
+#pragma unroll 1
+           while ((any = __ballot_sync(0xffffffffu, hits != 0u)) != 0u) {
+             const int at = near_n + __popc(any & ((1u << lane) - 1u));
+             if (hits && at < SP_NEAR) kept_near[at] = (u64)(place(j, __ffs(hits) - 1) - skip);
+             hits &= hits - 1;
+             near_n += __popc(any);
+           }
+         });
+    __syncwarp();
+    if (near_n > SP_NEAR) {
+      each(see, got);
+      return;
     }
+#pragma unroll 1
+    for (int e0 = n0 + lane; e0 < near_n; e0 += 128) {
+      int index[4];
+      T v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) index[i] = e0 + 32 * i < near_n ? (int)kept_near[e0 + 32 * i] : 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = __ldg(row + index[i]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (e0 + 32 * i < near_n) kept_near[e0 + 32 * i] = (u64)__float_as_uint(clean(In<DT>::f(v[i]))) << 32 | (uint32_t)index[i];
+    }
+#pragma unroll 1
+    for (int e = n0 + lane; e < near_n; e += 32) {
+      const uint32_t index = (uint32_t)kept_near[e];
+      if (!got(__uint_as_float((uint32_t)(kept_near[e] >> 32)), (int)index)) kept_near[e] = (u64)0x7fc00000u << 32 | index;
+    }
+    __syncwarp();
   };
 
   // --------------------------------------------------------- maximum, minimum
@@ -238,7 +286,6 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
   }
   for (int i = tid; i < SP_BINS; i += SP_THREADS) sh.count[i] = sh.lo[i] = sh.hi[i] = 0u;
   if (tid == 0) sh.listed = 0;
-  if (STREAM && lane == 0) sh.near_n[warp] = 0;
   float mx = -INFINITY, mn = INFINITY;  // mn: of those above -inf
   each(
       [&](float v) {
@@ -287,6 +334,29 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
     const float d = e - mx;  // (a NaN or an infinite d gives NaN or -inf, and so 0)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaxf(fmaf(d, f1, d * f2), -150.0f)));
     return __float2ull_rn(e * SP_ONE);  // (2^34 in the exponent's argument would cost it four bits)
+  };
+  // weigh(x, y) adds two weights to zh 2^17 + zl without conversions to 64 bits, which run at a fraction of the other
+  // instructions' rate: w 2^17 is rounded to an integer by adding 1.5 2^23, the remainder, which is exact, times 2^17
+  // likewise, and together they are w 2^34 rounded to the nearest integer, as in weight().  What the sums of the bit
+  // patterns have of 1.5 2^23's comes off at the end.
+  constexpr float SHIFT = 12582912.0f;
+  const uint64_t mx2 = pk2(-mx, -mx), f1x2 = pk2(f1, f1), f2x2 = pk2(f2, f2), limb2 = pk2(131072.0f, 131072.0f);
+  const uint64_t shift2 = pk2(SHIFT, SHIFT), minus2 = pk2(-1.0f, -1.0f);
+  uint32_t zh = 0u, zl = 0u;
+  auto weigh = [&](float x, float y) {
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(SP_FAR));
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(SP_FAR));
+    const uint64_t d = add2(pk2(x, y), mx2);
+    float e0, e1, h0, h1, l0, l1;
+    upk2(fma2(d, f1x2, mul2(d, f2x2)), e0, e1);
+    const uint64_t e = pk2(ex2(fmaxf(e0, -150.0f)), ex2(fmaxf(e1, -150.0f))), h = fma2(e, limb2, shift2);
+    const uint64_t l = fma2(fma2(e, limb2, fma2(h, minus2, shift2)), limb2, shift2);
+    upk2(h, h0, h1), upk2(l, l0, l1);
+    zh += __float_as_uint(h0) + __float_as_uint(h1), zl += __float_as_uint(l0) + __float_as_uint(l1);
+  };
+  auto weighed = [&]() -> u64 {  // what a walk() over weigh() has added up
+    const uint32_t off = (uint32_t)((loads + STEP - 1) / STEP * STEP * VEC) * __float_as_uint(SHIFT);
+    return ((u64)(zh - off) << SP_LIMB) + (u64)(int64_t)(int32_t)(zl - off);
   };
   int turn = 0;
   // The cluster's sum of a number per thread.
@@ -375,21 +445,19 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
   {
     // hits: what the histogram takes, or a greedy row's largest
     const float low = greedy ? mx : by_k || by_p ? mx - reach - fabsf(mx) * 2.4e-7f : INFINITY;
-    each(
-        [&](float v) {
-          z += weight(v);
-          return v >= low;
-        },
-        [&](float v, int index) {
-          if (greedy) first = min(first, index);
-          else if (in_band(v)) {
-            add(v);
-            keep_near(v, index);
-          }
-        });
-    __syncwarp();
-    have_near = __syncthreads_and(STREAM && sh.near_n[warp] <= SP_NEAR && (by_k || by_p));
-    near_reach = reach;
+    auto hit = [&](float v, int index) {
+      if (greedy) first = min(first, index);
+      else if (in_band(v)) return add(v), true;
+      return false;
+    };
+    if constexpr (STREAM) {
+      take([&](float v) { return v >= low; }, weigh, hit);
+      z = weighed();
+      have_near = __syncthreads_and(near_n <= SP_NEAR && (by_k || by_p));
+      near_reach = reach;
+    } else {
+      each([&](float v) { z += weight(v); return v >= low; }, hit);
+    }
     first = __reduce_min_sync(0xffffffffu, first);
     if (lane == 0) sh.ipart[warp] = first;
     z = sp_block_sum<SP_THREADS>(z, sh.part);
@@ -450,16 +518,14 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
       for (int i = tid; i < SP_BINS; i += SP_THREADS) sh.count[i] = sh.lo[i] = sh.hi[i] = 0u;
       __syncthreads();
       const float upper = from < 0.0f ? INFINITY : mx - from + fabsf(mx) * 2.4e-7f, lower = mx - reach - fabsf(mx) * 2.4e-7f;
-      each([&](float v) { return v >= lower && v <= upper; },
-           [&](float v, int index) {
-             if (!in_band(v)) return;
-             add(v);
-             if (have_near && reach > near_reach) keep_near(v, index);
-           });
-      __syncwarp();
+      auto see = [&](float v) { return v >= lower && v <= upper; };
+      auto hit = [&](float v, int) { return in_band(v) ? add(v), true : false; };
       if (STREAM && have_near && reach > near_reach) {  // (bands follow one another)
-        have_near = __syncthreads_and(sh.near_n[warp] <= SP_NEAR);
+        take(see, [](float, float) {}, hit);
+        have_near = __syncthreads_and(near_n <= SP_NEAR);
         near_reach = reach;
+      } else {
+        each_near(reach <= near_reach, see, hit);
       }
       barrier();
       return merge();
