@@ -121,11 +121,11 @@ __device__ __forceinline__ int sp_find_bin(SampleShared& sh, const T* v, double 
   return sh.found;
 }
 
-// STREAM: one CTA per row, which reads it anew for each pass (1024 threads, one CTA on an SM: the rows under way then fit
+// STREAM: CTAs that read their part anew for each pass (1024 threads, one CTA on an SM: the rows under way then fit
 // L2; with two they did not, and 512 rows of 131072 fp32 took 277 us); else a cluster's CTAs hold it.
 constexpr int SP_HELD_THREADS = 512, SP_STREAM_THREADS = 1024;
 constexpr int SP_NEAR = 640;  // logits of a band that a warp keeps (160 KB in all); more: the row is read again instead
-template <int DT, bool STREAM>
+template <int DT, bool STREAM, bool ALONE>
 __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, STREAM ? 1 : 2)
     sample_kernel(SampleArgs a, int loads) {
   constexpr int SP_THREADS = STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, SP_WARPS = SP_THREADS / 32;
@@ -137,10 +137,10 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
   static_assert(sizeof(SampleShared) % 16 == 0, "what follows is read 16 bytes at a time");
   uint4* held = reinterpret_cast<uint4*>(smem + sizeof(SampleShared));  // [warp][loads][lane]
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = STREAM ? 1 : (int)cluster.num_blocks(), rank = STREAM ? 0 : (int)cluster.block_rank();
-  auto peer = [&](int c) -> SampleShared& { return STREAM ? sh : *cluster.map_shared_rank(&sh, c); };
+  const int C = ALONE ? 1 : (int)cluster.num_blocks(), rank = ALONE ? 0 : (int)cluster.block_rank();
+  auto peer = [&](int c) -> SampleShared& { return ALONE ? sh : *cluster.map_shared_rank(&sh, c); };
   auto barrier = [&]() {
-    if (STREAM || C == 1) __syncthreads();
+    if (ALONE || C == 1) __syncthreads();
     else cluster.sync();
   };
   const int r = (int)(blockIdx.x / C), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -240,18 +240,15 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
     const int n0 = near_n;
     walk([&](float x, float y) { also(x, y); return (see(x) ? 1u : 0u) | (see(y) ? 2u : 0u); },
          [&](uint32_t hits, int j) {
-           if (!inner) {
 #pragma unroll 1
-             for (int i = 0; i < STEP * VEC; ++i)
-               if (!real(j, i)) hits &= ~(1u << i);
-           }
-           unsigned any;
-#pragma unroll 1
-           while ((any = __ballot_sync(0xffffffffu, hits != 0u)) != 0u) {
-             const int at = near_n + __popc(any & ((1u << lane) - 1u));
-             if (hits && at < SP_NEAR) kept_near[at] = (u64)(place(j, __ffs(hits) - 1) - skip);
+           while (__ballot_sync(0xffffffffu, hits != 0u) != 0u) {
+             const int i = __ffs(hits) - 1;
+             const bool hit = hits != 0u && (inner || real(j, i));
+             const unsigned all = __ballot_sync(0xffffffffu, hit);
+             const int at = near_n + __popc(all & ((1u << lane) - 1u));
+             if (hit && at < SP_NEAR) kept_near[at] = (u64)(place(j, i) - skip);
              hits &= hits - 1;
-             near_n += __popc(any);
+             near_n += __popc(all);
            }
          });
     __syncwarp();
@@ -538,7 +535,10 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
         u64 sn = 0, sw = 0;
         for (int i = tid; i < SP_BINS; i += SP_THREADS) sn += sh.total[i], sw += sh.mass[i];
         base_n += sp_block_sum<SP_THREADS>(sn, sh.part), base_w += sp_block_sum<SP_THREADS>(sw, sh.part);
-        if (!(merged = merged && band(reach, fminf(full, reach * 1.15f)))) return SP_BINS;
+        // how much further: counts grow by about e^1.4 for a unit of x, or less
+        const double more = by_mass ? 1.0 : target / (double)(base_n + 1);
+        const float further = more < 2.0 ? 1.15f : more < 8.0 ? 1.3f : 1.6f;
+        if (!(merged = merged && band(reach, fminf(full, reach * further)))) return SP_BINS;
       }
     };
     int listed_bin = -1, listed_from = 0, n = 0;  // the bins that are listed
@@ -736,9 +736,15 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
   });
 }
 
-// Many rows, one CTA each: its time is its instructions (about 35 a logit), and no CTA waits for another.  Few rows: a
-// cluster of CTAs each, as many as fill the card's 2 x 148 places but at most 8 unless the row needs more, since every
-// exchange over the cluster costs about a microsecond.
+// A row is held by a cluster of CTAs of 512 threads, two to an SM, or streamed by CTAs of 1024 threads, one to an SM.
+// Times in us with top_k and top_p, bf16, held / streamed by 1, 2, 4 CTAs:
+//   rows x V      16 x 100003         36 x 100003        64 x 32000         64 x 131072        148 x 131072
+//                 29 / 60, 43, 37     46 / 58, 43, 62    37 / 34, 35, 47    59 / 55, 39, 58    130 / 61, 75
+// Held is the shortest way while few CTAs are needed (up to 128; rows that one CTA holds always: 148 x 8000 31 / 33):
+// the row is read once, at the price of less room for anything else.  Then as many CTAs hold a row as there is room for, but at most 8
+// unless it needs more, since every exchange over the cluster costs about a microsecond.  Streamed rows get a cluster
+// while all of them run at the same time; from 196608 logits on two CTAs in any case, since the lists of one do not
+// hold the logits near the maximum (148 x 256000: 149 / 127 us with 1 / 2).
 template <int DT>
 int launch_sample(const SampleArgs& a, cudaStream_t st) {
   constexpr int VEC = DT == FP4_DT_F32 ? 4 : 8;
@@ -748,14 +754,15 @@ int launch_sample(const SampleArgs& a, cudaStream_t st) {
   const int most = DT == FP4_DT_F32 ? 16384 : 28672;  // 64 or 56 KB: two CTAs on an SM
   int C = 1;
   while (C < SP_RANKS && C * most < n) C *= 2;
-  const bool stream = C > 1 && (int64_t)a.R * C > 296;
-  if (stream) C = 1;
-  else
+  const bool stream = C > 1 && (int64_t)a.R * C > 128;
+  if (stream) {
+    C = a.R <= 32 ? 4 : a.R <= 64 || n > 196608 ? 2 : 1;
+  } else
     while (C < 8 && (int64_t)a.R * C * 2 <= 296 && C * 4096 < n) C *= 2;
   const int threads = stream ? SP_STREAM_THREADS : SP_HELD_THREADS;
   const int per_load = C * threads * VEC, loads = (n + per_load - 1) / per_load;
   const size_t smem = sizeof(SampleShared) + (stream ? (size_t)32 * SP_NEAR * 8 : (size_t)loads * threads * 16);
-  auto* fn = stream ? sample_kernel<DT, true> : sample_kernel<DT, false>;
+  auto* fn = !stream ? sample_kernel<DT, false, false> : C == 1 ? sample_kernel<DT, true, true> : sample_kernel<DT, true, false>;
   if (int e = set_smem_attr((const void*)fn, (int)sizeof(SampleShared) + (stream ? 32 * SP_NEAR * 8 : 73728), true)) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.R * C)), cfg.blockDim = dim3(threads);
