@@ -5,7 +5,7 @@
 // columns of transposed products, so that few rows cost few columns:
 //   S^T[key][row] = K^ Q^^T         tcgen05 kind::mxf4nvf4, the cache's codes and scales as they are
 //   O^T[d][row]  += V^^T[d][key] W[key][row]   tcgen05 kind::f16
-// with x = S scaling log2(e) + log2(g_v), W = 2^(x - m + 12) and, per row, m a
+// with x = S scaling log2(e) + log2(g_v), W = 2^(x - m + 9) and, per row, m a
 // running maximum of x.  Folding V's per-token scale g_v into the exponent keeps
 // W within fp16 whatever the values' sizes, and leaves code * scale for V^,
 // exact in fp16.  The row sum is l = sum W / g_v, in fp32.
@@ -83,9 +83,9 @@ struct PrepArgs {
   int NB, mask_blocks;
 };
 
-// Blocks [0, B*N): a block quantizes a query token (one g over its Hq * D channels).  Then mask_blocks blocks: a
-// warp per (row, node j) turns the mask's column j into bits over the nodes i that see it.  The last block lists
-// the rows and the tiles before each.
+// A launch's time (a few hundred tokens at most).  Blocks [0, B*N): a block quantizes a query token (one g over its
+// Hq * D channels).  Then mask_blocks blocks: a warp per (row, node j) turns the mask's column j into bits over the
+// nodes i that see it.  The last block lists the rows and the tiles before each.
 constexpr int PREP_THREADS = 256;
 template <int DT, bool VEC, int NBLK>
 __global__ void __launch_bounds__(PREP_THREADS) paged_prep_kernel(AttnArgs a, PrepArgs p) {
@@ -267,6 +267,9 @@ struct Share {
 // one walker that hands on what the others need through the stage, and apart what is rare (a moved maximum, masks,
 // an entry's end).  Then their number: a softmax warp's waits, arrivals and addresses cost about 210 a tile, its
 // 16 rows and 32 keys only 90, hence tiles of 256 keys and as many rows per warp as its registers hold.
+// With 64 rows it is about 10300 warp instructions a tile, 2500 of them V's widening and 1400 the exponentials.
+// Measured, all three kernels: 8 x 32768 keys, 8 heads, 8 rows: 99 us, 3.1 TB/s of 304 MB (46 us at a plain copy's
+// rate); 2 x 65536 keys, 8 heads, 512 rows: 554 us, 250 TFLOP/s in O^T (83 us at the fp16 rate of a large product).
 constexpr uint32_t KC = TK * PG_ROW, KS = TK * PG_SF, KG = TK * 4;
 constexpr uint32_t O_VC = KC, O_KS = 2 * KC, O_VS = O_KS + KS, O_KG = O_VS + KS, O_VG = O_KG + KG;
 constexpr uint32_t STAGE = O_VG + KG;  // K codes, V codes, K scales, V scales, K g, V g: 38 KB
@@ -1010,7 +1013,8 @@ __global__ void __launch_bounds__(Cfg<NB, PL>::THREADS, 1)
 // ------------------------------------------------------------------- joining
 // A block per (8 rows, row tile and KV head, b), a warp per row: O = sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i over
 // the CTAs that had tiles of the list entry, in their order.  Entries that one CTA did are already out; rows
-// without a tile are 0.
+// without a tile are 0.  A launch's time; done by the attention kernel's last CTA of an entry instead, it took longer
+// (6 x 27 nodes: 69 us in all instead of 55): one CTA's warps then join 64 rows at the end.
 template <int NB, int DT>
 __global__ void __launch_bounds__(256) paged_join_kernel(AttnArgs a, int grid_max) {
   pdl_wait();
@@ -1073,8 +1077,10 @@ __global__ void __launch_bounds__(256) paged_join_kernel(AttnArgs a, int grid_ma
 }
 
 // --------------------------------------------------------------------- host
-// Rows of a tile: the fewest tiles that hold all rows, as each of them reads the keys again and widens V again.
-// fp32 outputs keep W as two planes and O in registers, which leaves room for 32.
+// Rows of a tile: the fewest tiles that hold all rows, as each of them reads the keys again and widens V again (32 rows
+// of 4 x 2000 keys and 8 heads: 24.5 us as one tile of 64, 26.6 as two of 16), but no more than need be, as a tile's
+// exponentials are made for all of them (8 rows, 8 x 32768 keys: 99.6 us with tiles of 16, 123 with 64).  fp32
+// outputs keep W as two planes and O in registers, which leaves room for 32.
 int rows_per_tile(int64_t rows, bool fp32) { return rows <= 16 ? 16 : fp32 ? 32 : 64; }
 
 struct Layout {

@@ -12,8 +12,13 @@
 // Few rows: a cluster of CTAs reads a row once and holds it in shared memory; the
 // CTAs exchange their maxima, sums, histograms and the bin's logits over
 // distributed shared memory, and each draws the same conclusions from them.  Many rows: one
-// CTA per row goes over it twice, the second time mostly in L2, and keeps the logits near the
-// maximum, which are what the rest needs, in shared memory.
+// CTA per row, or a cluster of two or four, goes over it twice, the second time mostly in L2, and
+// keeps the logits near the maximum, which are what the rest needs, in shared memory.
+//
+// One row of 32000: 16 us, a chain of about a dozen exchanges and barriers.  512 rows of 131072 fp32 under
+// top_p: 183 us, 1.5 TB/s (41 us at a plain copy's rate).  There the first pass (maximum) runs at the
+// memory's rate and is a fifth of a row's time; the second (weights, sum, histogram), half of it, is bound
+// by instructions (about 16 per logit, half of them for the weight); what follows by latencies.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <stdint.h>

@@ -7,9 +7,9 @@ the rounding of p to one fp16 (2^-12; fp32 outputs: two fp16, 2^-22) and the
 error of the exponent, whose argument |S| log2(e) has a few 32-bit roundings
 (2^-21 max|S| log2(e) covers three), doubled for the sum in the denominator.
 The products p g_v (g_v: the token's global scale, at least its |v|) are held
-in fp16 relative to the row's largest: f = 2^-36 is half of fp16's smallest step
-under a scale of 2^12 that the running maximum keeps to within 2^3 up or down of
-exact; T tokens add up to T f of the largest.
+in fp16, scaled so that the row's largest is 2^9 to 2^15: half of fp16's smallest
+step is then 2^-34 to 2^-40 of it.  f = 2^-36 a token, since T such roundings do
+not all go one way; they add up to T f of the largest.
 """
 import math
 
