@@ -156,6 +156,34 @@ def test_nan_in_masked_places(rows, dtype):
         assert (many[0] >= 20000).all() and torch.isfinite(x.gather(1, many[0][:, None])).all()
 
 
+@pytest.mark.parametrize("kind", ["normal", "steps", "peaks"])
+@pytest.mark.parametrize("R,V,dtype", [(20, 131072, torch.float32), (40, 60001, torch.float32), (70, 100003, torch.bfloat16),
+                                       (130, 200001, torch.float16), (160, 33333, torch.bfloat16)])
+def test_many_long_rows_like_single_ones(R, V, dtype, kind):
+    """Rows that are not held on chip give what each gives alone, to the bit; the first ones what the definition says."""
+    from fp4_attn_b200.sampling import sample
+    if kind == "normal":
+        x, u = logits(R, V, dtype, seed=V + R)
+    else:
+        g = torch.Generator(device=DEV).manual_seed(V - R)
+        u = torch.rand(R, generator=g, device=DEV)
+        if kind == "steps":  # many equal logits
+            x = torch.randint(-3, 4, (R, V), generator=g, device=DEV).to(dtype)
+        else:  # a few far above the rest, which top_k goes down to
+            x = torch.randn(R, V, generator=g, device=DEV)
+            x[:, ::V // 5] += 30.0
+            x = x.to(dtype)
+    x[:, V // 2:V // 2 + 100] = float("-inf")
+    r = torch.arange(R, device=DEV)
+    kw = dict(T=(0.3 * (r % 8)).float(), k=(r * 53 % 400 - 20).int(), p=(1.06 - 0.11 * (r % 7)).float(), m=(0.02 * (r % 3)).float())
+    run(x[:12], u[:12], **{a: b[:12] for a, b in kw.items()})
+    tok, lp = sample(x, u, temperature=kw["T"], top_k=kw["k"], top_p=kw["p"], min_p=kw["m"])
+    for i in range(R):
+        s = slice(i, i + 1)
+        t1, l1 = sample(x[s], u[s], temperature=kw["T"][s], top_k=kw["k"][s], top_p=kw["p"][s], min_p=kw["m"][s])
+        assert torch.equal(tok[s], t1) and torch.equal(lp[s], l1), i
+
+
 def test_strides_shapes_and_streams():
     from fp4_attn_b200.sampling import sample
     x, u = logits(6, 777, torch.bfloat16, seed=3)
