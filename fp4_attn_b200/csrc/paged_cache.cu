@@ -7,7 +7,7 @@
 // integer reference counts, whose order does not matter.
 //
 // Few tokens are bound by launches (13 tokens of 8 sequences: truncate, append,
-// compact and gather are six launches, 27 us, 2.4 us' worth of bytes), many by bytes
+// compact and gather are six launches, 23 us, 2.4 us' worth of bytes), many by bytes
 // and by the quantizer's instructions: the data kernels read and write whole
 // 16-byte or 8-byte runs of a (token, head) row.
 #include <stdint.h>
@@ -170,7 +170,8 @@ struct AppendArgs {
 // A warp per (token, K or V): the token's blocks are quantized under one g and written to its slot.  They stay in
 // registers between the maximum and the codes, so that a token is read once.  3 x 8192 tokens of 8 heads, bf16: 35 us,
 // 3.7 TB/s of the 129 MB that go in and out; bound by instructions (22.6 million of a warp), which is why products
-// and roundings go in pairs (with gather below, 95 us one by one, 80 in pairs).
+// and roundings go in pairs (with gather below, 95 us one by one, 80 in pairs,
+// when that still had four tokens a thread).
 template <int DT, bool VEC, int NB>
 __global__ void __launch_bounds__(256) append_quant_kernel(fp4paged_cache c, const int32_t* seqs, AppendArgs a) {
   using E = typename In<DT>::T;
@@ -191,8 +192,8 @@ __global__ void __launch_bounds__(256) append_quant_kernel(fp4paged_cache c, con
         live = t < w.count[b];
         if (!live) return false;
         const int pos = w.start[b] + t;
-        page = c.page_table[(int64_t)pg_seq(c, seqs, b) * c.max_pages + pos / P];
-        slot = pos % P;
+        page = c.page_table[(int64_t)pg_seq(c, seqs, b) * c.max_pages + (pos >> (__ffs(P) - 1))];  // P is a power of 2
+        slot = pos & (P - 1);
         codes = (kv ? c.v_codes : c.k_codes) + (page * H * P + slot) * PG_ROW;
         scales = (kv ? c.v_scales : c.k_scales) + (page * H * P + slot) * PG_SF;
         return true;
@@ -416,14 +417,16 @@ __global__ void __launch_bounds__(256) fork_copy_kernel(fp4paged_cache c) {
 
 // ------------------------------------------------------------------ gather
 // A thread per block of 16 channels of GT tokens, 32 apart: 8 code bytes, a scale byte and g in, 16 values out.  A
-// token's data is three trips to memory away (length, page, bytes), so the tokens' trips are made together: 32 us for
-// 3 x 8192 tokens of 8 heads, 4.0 TB/s of 129 MB (46 us with one token a thread).
-constexpr int GT = 4;
+// token's data is three trips to memory away (length, page, bytes), so two tokens' trips are made together, and few
+// registers leave room for many warps: 3 x 8192 tokens of 8 heads, 129 MB, with append 71.8 us (four tokens a thread 77.6,
+// one 72.2), about 28 of them here, 4.6 TB/s.
+constexpr int GT = 2;
 template <int DT>
 __global__ void __launch_bounds__(256) gather_kernel(fp4paged_cache c, void* k_out, void* v_out, const int32_t* seqs,
                                                      int T) {
   using E = typename In<DT>::T;
   const int H = c.num_kv_heads, P = c.page_size, bh = blockIdx.y, b = bh / H, h = bh % H, kv = blockIdx.z;
+  const int shift = __ffs(P) - 1;  // P is a power of 2
   const int t0 = blockIdx.x * 32 * GT + (threadIdx.x >> 3), j = threadIdx.x & 7;
   const int s = pg_seq(c, seqs, b), len = s < 0 ? 0 : min(c.lens[s], T);
   const uint8_t *codes = kv ? c.v_codes : c.k_codes, *scales = kv ? c.v_scales : c.k_scales;
@@ -432,17 +435,17 @@ __global__ void __launch_bounds__(256) gather_kernel(fp4paged_cache c, void* k_o
 #pragma unroll
   for (int i = 0; i < GT; ++i) {
     const int t = t0 + 32 * i;
-    page[i] = t < len ? c.page_table[(int64_t)s * c.max_pages + t / P] : -1;
+    page[i] = t < len ? c.page_table[(int64_t)s * c.max_pages + (t >> shift)] : -1;
   }
   uint2 w[GT];
   float sc[GT], g[GT];
 #pragma unroll
   for (int i = 0; i < GT; ++i) {
-    const int slot = (t0 + 32 * i) % P;
-    const int64_t row = (page[i] * H + h) * P + slot;
+    const int slot = (t0 + 32 * i) & (P - 1);
+    const int64_t row = ((page[i] * H + h) << shift) + slot;
     w[i] = page[i] >= 0 ? __ldg(reinterpret_cast<const uint2*>(codes + row * PG_ROW) + j) : make_uint2(0u, 0u);
     sc[i] = page[i] >= 0 ? e4m3_to_f32(__ldg(scales + row * PG_SF + j)) : 0.0f;
-    g[i] = page[i] >= 0 ? __ldg(gs + page[i] * P + slot) : 0.0f;
+    g[i] = page[i] >= 0 ? __ldg(gs + (page[i] << shift) + slot) : 0.0f;
   }
 #pragma unroll
   for (int i = 0; i < GT; ++i) {
