@@ -418,8 +418,8 @@ __global__ void __launch_bounds__(256) fork_copy_kernel(fp4paged_cache c) {
 // ------------------------------------------------------------------ gather
 // A thread per block of 16 channels of GT tokens, 32 apart: 8 code bytes, a scale byte and g in, 16 values out.  A
 // token's data is three trips to memory away (length, page, bytes), so two tokens' trips are made together, and few
-// registers leave room for many warps: 3 x 8192 tokens of 8 heads, 129 MB, with append 71.8 us (four tokens a thread 77.6,
-// one 72.2), about 28 of them here, 4.6 TB/s.
+// registers leave room for many warps: 3 x 8192 tokens of 8 heads, 129 MB, with append 71.8 us (four tokens a thread
+// 77.6, one 72.2), about 28 of them here, 4.6 TB/s.
 constexpr int GT = 2;
 template <int DT>
 __global__ void __launch_bounds__(256) gather_kernel(fp4paged_cache c, void* k_out, void* v_out, const int32_t* seqs,
