@@ -26,8 +26,8 @@ constexpr int SCAN_PER_THREAD = 16;  // reference counts a thread reads at a tim
 // The int32 scratch of a cache.
 struct Work {
   int32_t* off;    // [max_seqs] first new page of a row, exclusive prefix
-  int32_t* start;  // [max_seqs] append: position of a row's first new token
-  int32_t* count;  // [max_seqs] append: its new tokens
+  int32_t* start;  // [max_seqs] append: position of a row's first new token; compact: tokens that the row ends with
+  int32_t* count;  // [max_seqs] append: its new tokens; compact: the row's error bits
   int32_t* total;  // [4] total[0]: new pages of the call
   int32_t* ids;    // [num_pages] the pages taken
   int32_t* from;   // [num_pages] fork: the page each is copied from
@@ -247,8 +247,8 @@ struct CompactArgs {
   int N;
 };
 
-// What a row's compaction does: base = its tail's first position, n kept tokens.  Returns the error bits (the
-// same in every block that asks); every thread of the block takes part.
+// What a row's compaction does: base = its tail's first position, n kept tokens.  Returns the error bits, the
+// same in every block that asks while no reference count changes; every thread of the block takes part.
 __device__ int compact_row(const fp4paged_cache& c, const CompactArgs& a, int b, int s, int& base, int& n) {
   const int len = c.lens[s], tail = a.tails ? a.tails[b] : a.N, P = c.page_size;
   const int32_t* keep = a.keep + (int64_t)b * a.N;
@@ -271,13 +271,21 @@ __device__ int compact_row(const fp4paged_cache& c, const CompactArgs& a, int b,
 
 // A block per (row, head, K or V) moves the kept tokens of its head down, 64 at a time: all of a chunk is read
 // before any of it is written.  keep is increasing, so token j moves from keep[j] >= j, and what later chunks
-// read lies past everything that earlier ones wrote.
+// read lies past everything that earlier ones wrote.  The row's verdict goes to the scratch: the next kernel lowers
+// reference counts, of pages that other rows of the call hold too, so it cannot come to one of its own.
 constexpr int MOVE_TOKENS = 64;
 __global__ void __launch_bounds__(4 * MOVE_TOKENS) compact_move_kernel(fp4paged_cache c, CompactArgs a) {
   const int b = blockIdx.x, h = blockIdx.y, kv = blockIdx.z, s = pg_seq(c, a.seqs, b);
-  if (s < 0) return;
+  const Work w = work_of(c);
+  const bool tells = h == 0 && kv == 0 && threadIdx.x == 0;
+  if (s < 0) {
+    if (tells) w.count[b] = PG_BAD_SEQ;
+    return;
+  }
   int base, n;
-  if (compact_row(c, a, b, s, base, n)) return;
+  const int err = compact_row(c, a, b, s, base, n);
+  if (tells) w.start[b] = base + n, w.count[b] = err;
+  if (err) return;
   const int P = c.page_size, H = c.num_kv_heads;
   const int32_t* row = c.page_table + (int64_t)s * c.max_pages;
   const int32_t* keep = a.keep + (int64_t)b * a.N;
@@ -310,19 +318,16 @@ __global__ void __launch_bounds__(4 * MOVE_TOKENS) compact_move_kernel(fp4paged_
   }
 }
 
-__global__ void __launch_bounds__(128) compact_drop_kernel(fp4paged_cache c, CompactArgs a) {
-  const int b = blockIdx.x, s = pg_seq(c, a.seqs, b);
-  if (s < 0) {
-    if (threadIdx.x == 0) atomicOr(c.status, PG_BAD_SEQ);
-    return;
-  }
-  int base, n;
-  const int old = c.lens[s], err = compact_row(c, a, b, s, base, n);
+__global__ void __launch_bounds__(128) compact_drop_kernel(fp4paged_cache c, const int32_t* seqs) {
+  const Work w = work_of(c);
+  const int b = blockIdx.x, err = w.count[b];
   if (err) {
     if (threadIdx.x == 0) atomicOr(c.status, err);
     return;
   }
-  drop_pages(c, s, old, base + n);
+  const int s = pg_seq(c, seqs, b), old = c.lens[s];
+  __syncthreads();  // every thread has read lens[s]
+  drop_pages(c, s, old, w.start[b]);
 }
 
 // -------------------------------------------------------------------- fork
@@ -554,11 +559,10 @@ extern "C" int fp4paged_compact(const fp4paged_cache* cache, const int32_t* keep
   if (!counts || (N > 0 && !keep)) return set_error(FP4ATTN_ERR_ARG, "keep or counts is null");
   const CompactArgs a{keep, counts, tails, seqs, N};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (N > 0) {
-    compact_move_kernel<<<dim3(B, cache->num_kv_heads, 2), 4 * MOVE_TOKENS, 0, st>>>(*cache, a);
-    if (int e = check_launch("compact_move_kernel")) return e;
-  }
-  compact_drop_kernel<<<B, 128, 0, st>>>(*cache, a);
+  const dim3 grid = N > 0 ? dim3(B, cache->num_kv_heads, 2) : dim3(B);  // (N 0: nothing to move, a verdict all the same)
+  compact_move_kernel<<<grid, 4 * MOVE_TOKENS, 0, st>>>(*cache, a);
+  if (int e = check_launch("compact_move_kernel")) return e;
+  compact_drop_kernel<<<B, 128, 0, st>>>(*cache, seqs);
   return check_launch("compact_drop_kernel");
 }
 
