@@ -149,6 +149,8 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
     else cluster.sync();
   };
   const int r = (int)(blockIdx.x / C), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // this CTA runs; waited for before the first access to another one's memory
+  if constexpr (!ALONE) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
   // A warp has consecutive positions, VEC per lane and load.  Positions count from the 16-byte boundary at or below
   // the row, so that loads are aligned whatever the row's start.
@@ -303,6 +305,7 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
   }
   if (lane == 0) sh.fpart[0][warp] = mx, sh.fpart[1][warp] = mn;
   __syncthreads();
+  if constexpr (!ALONE) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // all CTAs have started
   if (warp == 0) {
     mx = sh.fpart[0][lane & (SP_WARPS - 1)], mn = sh.fpart[1][lane & (SP_WARPS - 1)];
 #pragma unroll
