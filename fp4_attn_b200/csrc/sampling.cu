@@ -436,6 +436,8 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
   const float full = fminf(24.6f * temp, mx - mn);  // weights further away are 0
   const float near = full <= 8.0f ? full : fminf(fmaxf(7.0f * temp, 7.0f), full);
   float from = -1.0f, reach = near, per = reach > 0.0f ? (float)SP_BINS / reach : 0.0f;  // the band (from, reach] below mx
+  // more than the roundings of mx - distance and of mx - v, for a v near it, come to (2^-24 of |mx| + distance each)
+  auto slack = [&](float distance) { return (fabsf(mx) + distance) * 4.8e-7f; };
   auto in_band = [&](float v) { return mx - v > from && mx - v <= reach; };
   auto bin_of = [&](float v) { return max(0, min(SP_BINS - 1, (int)((mx - v - fmaxf(from, 0.0f)) * per))); };
   auto add = [&](float v) {
@@ -449,7 +451,7 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
   int first = INT32_MAX;
   {
     // hits: what the histogram takes, or a greedy row's largest
-    const float low = greedy ? mx : by_k || by_p ? mx - reach - fabsf(mx) * 2.4e-7f : INFINITY;
+    const float low = greedy ? mx : by_k || by_p ? mx - reach - slack(reach) : INFINITY;
     auto hit = [&](float v, int index) {
       if (greedy) first = min(first, index);
       else if (in_band(v)) return add(v), true;
@@ -522,7 +524,7 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
       barrier();  // (the histograms have been read)
       for (int i = tid; i < SP_BINS; i += SP_THREADS) sh.count[i] = sh.lo[i] = sh.hi[i] = 0u;
       __syncthreads();
-      const float upper = from < 0.0f ? INFINITY : mx - from + fabsf(mx) * 2.4e-7f, lower = mx - reach - fabsf(mx) * 2.4e-7f;
+      const float upper = from < 0.0f ? INFINITY : mx - from + slack(from), lower = mx - reach - slack(reach);
       auto see = [&](float v) { return v >= lower && v <= upper; };
       auto hit = [&](float v, int) { return in_band(v) ? add(v), true : false; };
       if (STREAM && have_near && reach > near_reach) {  // (bands follow one another)
@@ -568,7 +570,7 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
       above_n = base_n + (all ? 0 : sn), above_w = base_w + (all ? 0 : sp_block_sum<SP_THREADS>(sw, sh.part));
       listed_bin = bin, listed_from = all ? 0 : bin;
       // (a range that surely has the bin, to pass over the others quickly)
-      const float wide = fabsf(mx) * 2.4e-7f, at0 = mx - fmaxf(from, 0.0f);
+      const float wide = slack(reach), at0 = mx - fmaxf(from, 0.0f);
       const float hi = listed_from ? at0 - (float)(listed_from - 1) / per + wide : INFINITY;
       const float lo = per > 0.0f ? at0 - (float)(bin + 2) / per - wide : -INFINITY;
       each_near(

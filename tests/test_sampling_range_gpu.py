@@ -35,3 +35,35 @@ def test_rows_held_by_clusters_on_a_busy_gpu():
     torch.cuda.synchronize()
     for j, (tok, lp) in got:
         assert torch.equal(tok, alone[j][0]) and torch.equal(lp, alone[j][1])
+
+
+def band_edge(seed):
+    """(max, T, a logit 7 T below the maximum up to rounding, in 32 bits) such that max - logit <= 7 T but logit is below
+    max - 7 T - |max| 2.4e-7."""
+    F = np.float32
+    rng = np.random.RandomState(seed)
+    while True:
+        mx, T = F(rng.uniform(0.05, 3.0)), F(rng.uniform(1.2, 3.0))
+        reach = F(F(7.0) * T)
+        low = F(F(mx - reach) - F(mx * F(2.4e-7)))
+        v = np.nextafter(low, F(-np.inf))
+        if F(mx - v) <= reach:
+            return mx, T, v
+
+
+@pytest.mark.parametrize("R,V", [(1, 3001), (40, 60001), (160, 60001)])
+def test_a_logit_at_a_bands_edge(R, V):
+    """top_k ends at a logit that lies on the first band's edge: it counts, and the next one is dropped."""
+    k = 40
+    x = np.full((R, V), -60.0, np.float32)
+    T = np.zeros(R, np.float32)
+    for r in range(R):
+        mx, T[r], v = band_edge(R + r)
+        x[r, 5:5 + k - 2] = mx - np.float32(0.5)
+        x[r, 2], x[r, 3] = mx, v
+        x[r, V - 7] = v - np.float32(0.01)  # the first that top_k drops, the last in index order
+    t = torch.from_numpy(x).to(DEV)
+    u = torch.full((R,), float(np.nextafter(np.float32(1), np.float32(0))), device=DEV)
+    from fp4_attn_b200.sampling import sample
+    tok, _ = sample(t, u, temperature=torch.from_numpy(T).to(DEV), top_k=k)
+    assert tok.tolist() == [5 + k - 3] * R
