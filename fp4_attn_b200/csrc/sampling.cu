@@ -250,7 +250,8 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
 #pragma unroll 1
            while (__ballot_sync(0xffffffffu, hits != 0u) != 0u) {
              const int i = __ffs(hits) - 1;
-             const bool hit = hits != 0u && (inner || real(j, i));
+             // (-inf that stands in for what a step has past the warp's loads is a hit where see() has no lower end)
+             const bool hit = hits != 0u && ((inner && j + STEP <= loads) || real(j, i));
              const unsigned all = __ballot_sync(0xffffffffu, hit);
              const int at = near_n + __popc(all & ((1u << lane) - 1u));
              if (hit && at < SP_NEAR) kept_near[at] = (u64)(place(j, i) - skip);

@@ -67,3 +67,31 @@ def test_a_logit_at_a_bands_edge(R, V):
     from fp4_attn_b200.sampling import sample
     tok, _ = sample(t, u, temperature=torch.from_numpy(T).to(DEV), top_k=k)
     assert tok.tolist() == [5 + k - 3] * R
+
+
+@pytest.mark.parametrize("R,V,dtype", [(1, 5000, torch.float32), (40, 60001, torch.float32), (100, 60001, torch.float32),
+                                       (200, 90001, torch.bfloat16)])
+def test_the_whole_range_of_logits(R, V, dtype):
+    """Logits down to the type's lowest value under a temperature of their size: no band ends above them."""
+    from fp4_attn_b200.sampling import sample
+    far = torch.finfo(dtype).min
+    g = torch.Generator(device=DEV).manual_seed(V)
+    x = (-1e38 - torch.rand(R, V, generator=g, device=DEV) * 2.4e38).clamp(min=far).to(dtype)
+    x[:, 7:9], x[:, 100:200], x[:, 30] = far, float("-inf"), -1e38
+    u = torch.rand(R, generator=g, device=DEV)
+    for kw in (dict(top_k=40), dict(top_p=0.7), dict(top_k=300, top_p=0.5)):
+        tok, lp = sample(x, u, temperature=3e38, **kw)
+        for r in range(0, R, 17):
+            d = x[r].double()
+            order = torch.sort(-d, stable=True).indices
+            p = torch.exp((d - d.max()) / float(np.float32(3e38)))[order]
+            n = kw.get("top_k", V)
+            eps = 56 * 2.0 ** -23 + V * 2.0 ** -35
+            fine = False
+            c = p[:n].cumsum(0)
+            sizes = [n] if "top_p" not in kw else [max(1, int((c - p[:n] < (kw["top_p"] + e) * c[-1]).sum())) for e in (-eps, eps)]
+            for m in range(sizes[0], sizes[-1] + 1):
+                q = torch.zeros(V, dtype=torch.float64, device=DEV).index_copy(0, order[:m], p[:m] / p[:m].sum())
+                t = q.cumsum(0)[int(tok[r])]
+                fine |= bool(q[int(tok[r])] > 0 and t - q[int(tok[r])] <= float(u[r]) + 2 * eps and t >= float(u[r]) - 2 * eps)
+            assert fine, (r, kw)
