@@ -327,9 +327,9 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
     return;
   }
   const float t0 = a.temperature ? a.temperature[r] : 1.0f, temp = t0 > 0.0f ? fmaxf(t0, 1e-30f) : 1.0f;
-  const bool greedy = !(t0 > 0.0f);
   const int k = a.top_k ? a.top_k[r] : 0;
   const float top_p = a.top_p ? a.top_p[r] : 1.0f, min_p = a.min_p ? a.min_p[r] : 0.0f;
+  const bool greedy = !(t0 > 0.0f) || !(min_p <= 1.0f);  // (min_p above 1: nothing is left but the first)
   const bool by_k = !greedy && k > 0 && k < a.V, by_p = !greedy && top_p < 1.0f;
   // w = 2^((x - max) log2(e) / T): the factor in two parts, so that the product is rounded once
   const double f = 1.4426950408889634 / (double)temp;
@@ -719,7 +719,7 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
   }
 
   // ----------------------------------------------------------------- the draw
-  const u64 least = (u64)ceil((double)fmaxf(fminf(min_p, 1.0f), 0.0f) * (double)SP_ONE);
+  const u64 least = (u64)ceil((double)fmaxf(min_p, 0.0f) * (double)SP_ONE);
   // (key 0 is below every logit's)
   const float edge = cut.key == 0u ? -INFINITY : logit_of(cut.key);
   auto kept = [&](float v, int index) -> u64 {

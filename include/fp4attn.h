@@ -415,7 +415,7 @@ int fp4paged_attention(const fp4paged_cache* cache, const void* q, int in_dtype,
  * ascending) a row keeps the first top_k[r] (<= 0: all), of those the
  * shortest prefix with a share of at least top_p[r] (>= 1: all), of those
  * the ones with a weight of at least min_p[r] of the largest; always the
- * first.  The token is the first kept index i (in index order) whose running
+ * first (above 1: only that).  The token is the first kept index i (in index order) whose running
  * sum exceeds floor(u * sum).  temperature <= 0: the lowest index of the
  * largest logit.  NaN counts as -inf, +inf as the largest finite value.
  * logprob[r] (may be NULL) = log softmax(x / temperature)[token], before the

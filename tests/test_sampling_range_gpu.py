@@ -95,3 +95,20 @@ def test_the_whole_range_of_logits(R, V, dtype):
                 t = q.cumsum(0)[int(tok[r])]
                 fine |= bool(q[int(tok[r])] > 0 and t - q[int(tok[r])] <= float(u[r]) + 2 * eps and t >= float(u[r]) - 2 * eps)
             assert fine, (r, kw)
+
+
+@pytest.mark.parametrize("R", [1, 200])
+@pytest.mark.parametrize("min_p", [1.5, float("inf"), float("nan")])
+def test_min_p_that_nothing_reaches_keeps_the_first(R, min_p):
+    """No weight is min_p times the largest: what is left is the first of the largest logits, whatever u; with min_p 1
+    all of the largest are kept."""
+    from fp4_attn_b200.sampling import sample
+    x, u = logits(R, 20000, torch.bfloat16, seed=R)
+    x[:, [77, 500, 19999]] = 40.0
+    u[0] = 0.9
+    for kw in ({}, dict(top_k=9), dict(top_p=0.9)):
+        tok, lp = sample(x, u, temperature=0.7, min_p=min_p, **kw)
+        assert (tok == 77).all()
+        want = -torch.logsumexp((x.double() - 40.0) / float(np.float32(0.7)), 1)
+        assert (lp.double() - want).abs().max() < 2.0 ** -21
+        assert int(sample(x, u, temperature=0.7, min_p=1.0, **kw)[0][0]) == 19999
