@@ -38,6 +38,10 @@ constexpr int TK = 256, HK = 128;  // keys of a tile, in two halves of 128 (an M
 // moved in every second tile, which costs several times a tile without.)
 constexpr float W_BIAS = 9.0f, W_SLACK = 6.0f;
 constexpr float GV_MIN = 7.888609052e-31f;  // 2^-100: V tokens below count as 0, so that 1/g_v sums stay finite
+// 2^-64, the g_v of a token that counts as 0.  It is in l = sum W / g_v as any other (from W's 2^-126 on: while the others'
+// g_v are below 2^38, whatever has a share of 2^-24 or more), and should not be what m follows, for then the others' W,
+// smaller by g_v, would be rounded away: with 1 those of g_v 2^-25 kept 8 bits and less.
+constexpr float GV_ZERO = 5.421010862e-20f;
 constexpr float L_SCALE = 0.0009765625f;    // 2^-10, for the same reason
 
 // A row of the call, as the first kernel found it.
@@ -750,7 +754,7 @@ __global__ void __launch_bounds__(Cfg<NB, PL>::THREADS, 1)
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         if (ti.pos + hf * HK + key >= ti.len) ak[hf] = 0.0f, lg[hf] = 1.0f;
-        const float gs = lg[hf] >= GV_MIN ? lg[hf] : 1.0f;  // 0 and NaN: V^ is 0 there
+        const float gs = lg[hf] >= GV_MIN ? lg[hf] : GV_ZERO;  // 0 and NaN: V^ is 0 there
         lg[hf] = lg[hf] != lg[hf] ? lg[hf] : lg2(gs), rg[hf] = rcp(gs) * L_SCALE;
       }
       ok = warp_wait(&s_full[k], (it >> 1) & 1, 0x60b) && ok;

@@ -224,7 +224,8 @@ def tree_attention(q: torch.Tensor, cache: PagedNVFP4Cache, mask: torch.Tensor |
     channels), QK^T runs on the FP4 tensor cores, softmax in fp32, and P is not
     quantized: blocks of P would run over sibling nodes, so that a token's
     output would depend on what else was drafted.  The output has q's dtype
-    unless out or out_dtype says otherwise.
+    unless out or out_dtype says otherwise.  V tokens whose largest value is
+    below 2^-100 count as 0.
 
     workspace: a device buffer of fp4paged_attention_workspace_size bytes,
     256-byte aligned (default: one that the cache keeps).

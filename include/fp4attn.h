@@ -400,7 +400,8 @@ int fp4paged_gather(const fp4paged_cache* cache, void* k_out, void* v_out, int o
  * of those, node j is visible to node i where mask[b*m_sB + i*m_sI + j*m_sJ]
  * is not 0 (NULL: j <= i).  counts [B] (NULL: N): row b has counts[b] <= N
  * nodes, its last tokens; further rows of out are 0, as is one that sees no
- * key. */
+ * key.  A V token with g below 2^-100 counts as 0 (its share of the softmax
+ * stays); next to such tokens values are held to T 2^-100, and below 2^38. */
 int64_t fp4paged_attention_workspace_size(int B, int Hq, int Hkv, int N);
 int fp4paged_attention(const fp4paged_cache* cache, const void* q, int in_dtype, int B, int Hq, int N, int64_t q_sB,
                        int64_t q_sH, int64_t q_sT, const uint8_t* mask, int64_t m_sB, int64_t m_sI, int64_t m_sJ,

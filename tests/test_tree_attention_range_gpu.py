@@ -36,15 +36,19 @@ def quantized(q):
     return torch.from_numpy(out).double().view(B, N, H, D).transpose(1, 2).to(DEV)
 
 
-def formula(q, c, b=0):
-    """(o, sum p |v|) [N, Hq, D] of sequence b under a causal mask, in 64 bits."""
+def formula(q, c, b=0, g0=0.0):
+    """(o, sum p |v|, T max(p g) with g0 for tokens without a value, max |S|) of sequence b under a causal mask, in 64 bits;
+    the first three [N, Hq, D]."""
     Hq, N = q.shape[1:3]
     L, G = int(c.lens[b]), Hq // c.num_kv_heads
-    k, v = (t[b].double().repeat_interleave(G, 0) for t in c.gather(L))
+    K, V = (t[b].double() for t in c.gather(L))
+    k, v = (t.repeat_interleave(G, 0) for t in (K, V))
     S = quantized(q)[b] @ k.transpose(1, 2) * D ** -0.5
+    smax = float(S.abs().max())
     S[:, :, L - N:].masked_fill_(torch.ones(N, N, dtype=torch.bool, device=DEV).triu(1), -math.inf)
     p = torch.softmax(S, -1)
-    return (p @ v).transpose(0, 1), (p @ v.abs()).transpose(0, 1)
+    top = L * (p * V.abs().amax((0, 2)).clamp(min=g0)).amax(-1)
+    return (p @ v).transpose(0, 1), (p @ v.abs()).transpose(0, 1), top.transpose(0, 1)[..., None], smax
 
 
 def ended():
@@ -81,5 +85,37 @@ def test_large_finite_scores(exponent, dtype, N, G):
         cache = cache_of(k, v)
         o = tree_attention(q, cache)
         ended()
-        ref, share = formula(q, cache)
+        ref, share, _, _ = formula(q, cache)
         assert (o[0].double() - ref).abs().le(U[dtype] * ref.abs() + E[dtype] * share + 2.0 ** -24).all(), (kind, exponent)
+
+
+# ------------------------------------------------- V tokens without a value
+@pytest.mark.parametrize("largest", [False, True])
+@pytest.mark.parametrize("exponent,dtype", [(0, torch.float32), (-10, torch.float16), (-10, torch.float32), (-25, torch.bfloat16),
+                                            (-25, torch.float32), (-40, torch.bfloat16), (-40, torch.float32),
+                                            (15, torch.float16), (40, torch.float32)])
+@pytest.mark.parametrize("N,G", [(1, 2), (9, 4)])
+def test_zero_values_among_small_ones(exponent, dtype, largest, N, G):
+    """Tokens whose V is 0 (or below 2^-100) take their share of the softmax and nothing else: the others' values keep
+    their precision, whatever their size, also where a token without a value has the largest score.  Such a token
+    counts as one of 2^-64 where m is made, which adds T f 2^-64 p to what W is rounded by."""
+    from fp4_attn_b200.paged_cache import tree_attention
+    T = 900
+    g = torch.Generator(device=DEV).manual_seed(exponent + 100)
+    k = torch.randn(1, 2, T, D, generator=g, device=DEV)
+    v = torch.randn(1, 2, T, D, generator=g, device=DEV) * 2.0 ** exponent
+    v[:, :, 5::7] = 0
+    v[:, :, 6::50] = 2.0 ** -110
+    v[:, :, :300] = 0  # a whole tile of them
+    q = 2.0 * torch.randn(1, 2 * G, N, D, generator=g, device=DEV)
+    if largest:  # node 0's own direction, at places without a value
+        for h in range(2):
+            k[0, h, [40, 5 + 7 * 100]] = q[0, h * G, 0] * 1.2
+    cache = cache_of(k, v)
+    o = tree_attention(q, cache, out_dtype=dtype)
+    ended()
+    ref, share, top, smax = formula(q, cache, g0=2.0 ** -64)
+    e = E[dtype] + 2.0 ** -20 * smax * 1.4427
+    tol = U[dtype] * ref.abs() + e * share + 2.0 ** -36 * top + 2.0 ** -24 * (dtype == torch.float16)
+    err = (o[0].double() - ref).abs()
+    assert (err <= tol).all(), float((err / tol).max())
