@@ -163,6 +163,7 @@ __global__ void __launch_bounds__(PREP_THREADS) paged_prep_kernel(AttnArgs a, Pr
         Row r;
         r.slot = pg_seq(a.c, p.seqs, b);
         r.len = r.slot < 0 ? 0 : a.c.lens[r.slot];
+        if (r.slot < 0) atomicOr(a.c.status, PG_BAD_SEQ);
         // a sequence with fewer tokens than nodes has only those
         r.n = min(r.len, p.counts ? max(0, min(p.counts[b], a.N)) : a.N);
         r.pad = 0;

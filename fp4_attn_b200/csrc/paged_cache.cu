@@ -434,6 +434,7 @@ __global__ void __launch_bounds__(256) gather_kernel(fp4paged_cache c, void* k_o
   const int shift = __ffs(P) - 1;  // P is a power of 2
   const int t0 = blockIdx.x * 32 * GT + (threadIdx.x >> 3), j = threadIdx.x & 7;
   const int s = pg_seq(c, seqs, b), len = s < 0 ? 0 : min(c.lens[s], T);
+  if (s < 0 && h == 0 && kv == 0 && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(c.status, PG_BAD_SEQ);
   const uint8_t *codes = kv ? c.v_codes : c.k_codes, *scales = kv ? c.v_scales : c.k_scales;
   const float* gs = kv ? c.v_g : c.k_g;
   int64_t page[GT];

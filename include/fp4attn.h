@@ -342,7 +342,8 @@ int fp4attn_decode_ex(const uint8_t* q_codes, const uint8_t* q_scales, const flo
  *   write to a shared page (a fork shortened into a page that was full: fork
  *   it with deep), 16 a sequence index out of range or a fork onto a sequence
  *   that is not empty.  An append or a fork that would set a bit changes
- *   nothing else; a compaction leaves that sequence alone.
+ *   nothing else; a compaction leaves that sequence alone; a gather and an
+ *   attention give zeros for its row.
  *   work: fp4paged_work_size(num_pages, max_seqs) int32 of scratch.
  * page_size 16, 32, 64 or 128; D 128; all buffers 16-byte aligned.  seqs [B]
  * names each row's sequence (distinct; NULL: row b is sequence b).
