@@ -27,7 +27,7 @@ constexpr int SCAN_PER_THREAD = 16;  // reference counts a thread reads at a tim
 struct Work {
   int32_t* off;    // [max_seqs] first new page of a row, exclusive prefix
   int32_t* start;  // [max_seqs] append: position of a row's first new token; compact: tokens that the row ends with
-  int32_t* count;  // [max_seqs] append: its new tokens; compact: the row's error bits
+  int32_t* count;  // [max_seqs] append: its new tokens; compact: the row's error bits; fork: a mark
   int32_t* total;  // [4] total[0]: new pages of the call
   int32_t* ids;    // [num_pages] the pages taken
   int32_t* from;   // [num_pages] fork: the page each is copied from
@@ -110,6 +110,15 @@ __device__ __forceinline__ int row_of(const int32_t* off, int B, int i) {
   return lo;
 }
 
+// Whether another row of the call names row b's sequence s: two rows would change one sequence at the same time.  The
+// block looks through all rows; every thread of it takes part.
+__device__ __forceinline__ bool named_twice(const int32_t* seqs, int B, int b, int s) {
+  bool twice = false;
+  if (seqs)
+    for (int j = threadIdx.x; j < B; j += blockDim.x) twice |= j != b && seqs[j] == s;
+  return __syncthreads_or(twice);
+}
+
 // ------------------------------------------------------------------ append
 __global__ void __launch_bounds__(PLAN_THREADS) append_plan_kernel(fp4paged_cache c, const int32_t* seqs,
                                                                    const int32_t* counts, int B, int T) {
@@ -119,6 +128,14 @@ __global__ void __launch_bounds__(PLAN_THREADS) append_plan_kernel(fp4paged_cach
   const int P = c.page_size;
   if (threadIdx.x == 0) err = 0;
   __syncthreads();
+  if (seqs) {  // no two rows name one sequence: each finds its own mark
+    for (int b = threadIdx.x; b < B; b += PLAN_THREADS)
+      if (const int s = pg_seq(c, seqs, b); s >= 0) w.off[s] = b;
+    __syncthreads();
+    for (int b = threadIdx.x; b < B; b += PLAN_THREADS)
+      if (const int s = pg_seq(c, seqs, b); s >= 0 && w.off[s] != b) atomicOr(&err, PG_BAD_SEQ);
+    __syncthreads();
+  }
   int need = 0;
   for (int b0 = 0; b0 < B; b0 += PLAN_THREADS) {
     const int b = b0 + threadIdx.x;
@@ -219,7 +236,8 @@ int launch_append(const fp4paged_cache& c, const int32_t* seqs, const AppendArgs
 }
 
 // ------------------------------------------------- truncate, release, compact
-// (a few integers per sequence: a launch's time)
+// (a few integers per sequence: a launch's time.)  Rows that name one sequence are refused, all of them: two blocks
+// would drop the same pages, the second one by what the first has left in the page table.
 // Sequence s keeps its first len tokens; the block drops the pages past them.
 __device__ __forceinline__ void drop_pages(const fp4paged_cache& c, int s, int old, int len) {
   const int P = c.page_size;
@@ -233,12 +251,11 @@ __device__ __forceinline__ void drop_pages(const fp4paged_cache& c, int s, int o
 
 __global__ void __launch_bounds__(128) truncate_kernel(fp4paged_cache c, const int32_t* lens, const int32_t* seqs) {
   const int s = pg_seq(c, seqs, blockIdx.x);
-  if (s < 0) {
+  const int old = s < 0 ? 0 : c.lens[s], len = lens ? max(0, min(lens[blockIdx.x], old)) : 0;
+  if (named_twice(seqs, gridDim.x, blockIdx.x, s) || s < 0) {  // (every thread has read lens[s])
     if (threadIdx.x == 0) atomicOr(c.status, PG_BAD_SEQ);
     return;
   }
-  const int old = c.lens[s], len = lens ? max(0, min(lens[blockIdx.x], old)) : 0;
-  __syncthreads();  // every thread has read lens[s]
   drop_pages(c, s, old, len);
 }
 
@@ -278,7 +295,7 @@ __global__ void __launch_bounds__(4 * MOVE_TOKENS) compact_move_kernel(fp4paged_
   const int b = blockIdx.x, h = blockIdx.y, kv = blockIdx.z, s = pg_seq(c, a.seqs, b);
   const Work w = work_of(c);
   const bool tells = h == 0 && kv == 0 && threadIdx.x == 0;
-  if (s < 0) {
+  if (named_twice(a.seqs, gridDim.x, b, s) || s < 0) {
     if (tells) w.count[b] = PG_BAD_SEQ;
     return;
   }
@@ -340,6 +357,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(fp4paged_cache 
   const Work w = work_of(c);
   const int P = c.page_size;
   if (threadIdx.x == 0) err = 0;
+  for (int r = threadIdx.x; r < n; r += PLAN_THREADS)
+    if (const int d = pg_seq(c, dst, r); d >= 0) w.count[d] = r;  // a mark: no two rows go to one sequence
   __syncthreads();
   int need = 0;
   for (int r0 = 0; r0 < n; r0 += PLAN_THREADS) {
@@ -348,7 +367,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(fp4paged_cache 
     if (r < n) {
       const int s = pg_seq(c, src, r), d = pg_seq(c, dst, r);
       int len = 0;
-      if (s < 0 || d < 0 || c.lens[d] != 0) atomicOr(&err, PG_BAD_SEQ);
+      if (s < 0 || d < 0 || c.lens[d] != 0 || w.count[d] != r) atomicOr(&err, PG_BAD_SEQ);
       else len = c.lens[s], m = (len + P - 1) / P - (deep ? 0 : len / P);
       w.start[r] = len;
     }

@@ -29,6 +29,9 @@ Errors that only the device can see (no free pages, a sequence longer than its
 row of the page table, ...) leave the cache as it was and set bits in
 ``status``; ``check()`` reads them (it waits for the GPU) and raises.
 
+``seqs`` of a call that changes sequences names each of them once (twice is
+such an error); ``gather`` and ``tree_attention`` may read one in several rows.
+
 Calls on one cache go to one stream, or are ordered by the caller.
 """
 from __future__ import annotations
@@ -43,7 +46,7 @@ HEAD_DIM = 128
 PAGE_SIZES = (16, 32, 64, 128)
 ERRORS = {1: "not enough free pages", 2: "a sequence is longer than its row of the page table",
           4: "a keep list is not increasing or leaves its tail", 8: "a write to a shared page (fork with deep=True)",
-          16: "a sequence index out of range, or a fork onto a sequence that is not empty"}
+          16: "a sequence index out of range, a sequence named twice, or a fork onto a sequence that is not empty"}
 
 
 class _Struct(ctypes.Structure):  # fp4paged_cache of include/fp4attn.h
@@ -129,7 +132,8 @@ class PagedNVFP4Cache:
     def append(self, k: torch.Tensor, v: torch.Tensor, seqs: torch.Tensor | None = None,
                counts: torch.Tensor | None = None) -> None:
         """Quantize T new tokens per row, k and v [B, H, T, D] (post-RoPE K), and store them behind sequence
-        seqs[b] (default: b); counts [B] int32: only the first counts[b] tokens of row b."""
+        seqs[b] (int32 [B], each sequence once; default: b); counts [B] int32: only the first counts[b] tokens of row
+        b."""
         shape, device = k.shape, self.device
         if k.device != device or v.device != device:
             _lib.require_cuda(k, v)
@@ -149,19 +153,20 @@ class PagedNVFP4Cache:
                    self._rows(seqs, B), None if counts is None else _int32("counts", counts, (B,), device))
 
     def truncate(self, lens: torch.Tensor, seqs: torch.Tensor | None = None) -> None:
-        """Row b keeps its first lens[b] tokens (int32 [B]) if it has more; pages nobody holds become free."""
+        """Row b (sequence seqs[b], each once) keeps its first lens[b] tokens (int32 [B]) if it has more; pages nobody
+        holds become free."""
         B = lens.shape[0]
         self._call("fp4paged_truncate", _int32("lens", lens, (B,), self.device), self._rows(seqs, B), B)
 
     def release(self, seqs: torch.Tensor | None = None) -> None:
-        """Empty the sequences seqs (int32; default: all) and free the pages that nobody else holds."""
+        """Empty the sequences seqs (int32, each once; default: all) and free the pages that nobody else holds."""
         B = self.max_seqs if seqs is None else seqs.shape[0]
         self._call("fp4paged_truncate", None, self._rows(seqs, B), B)
 
     def compact(self, keep: torch.Tensor, counts: torch.Tensor, seqs: torch.Tensor | None = None,
                 tails: torch.Tensor | None = None) -> None:
         """Of the last tails[b] tokens (default: N) of row b keep those listed in keep[b, :counts[b]] (int32 [B, N],
-        increasing, 0 = the tail's first token), moved together; the rest is dropped."""
+        increasing, 0 = the tail's first token), moved together; the rest is dropped.  seqs: each sequence once."""
         if keep.dim() != 2:
             raise ValueError("keep must be [B, N]")
         B, N = keep.shape

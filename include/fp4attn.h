@@ -340,13 +340,15 @@ int fp4attn_decode_ex(const uint8_t* q_codes, const uint8_t* q_scales, const flo
  *   2 a sequence longer than its row of the page table, 4 a keep list that is
  *   not increasing or leaves its tail, 8 an append or a compaction that would
  *   write to a shared page (a fork shortened into a page that was full: fork
- *   it with deep), 16 a sequence index out of range or a fork onto a sequence
- *   that is not empty.  An append or a fork that would set a bit changes
- *   nothing else; a compaction leaves that sequence alone; a gather and an
- *   attention give zeros for its row.
+ *   it with deep), 16 a sequence index out of range, a sequence named twice by
+ *   a call that changes it, or a fork onto a sequence that is not empty.  An
+ *   append or a fork that would set a bit changes nothing else; a compaction
+ *   or a truncation leaves that sequence alone; a gather and an attention give
+ *   zeros for its row.
  *   work: fp4paged_work_size(num_pages, max_seqs) int32 of scratch.
  * page_size 16, 32, 64 or 128; D 128; all buffers 16-byte aligned.  seqs [B]
- * names each row's sequence (distinct; NULL: row b is sequence b).
+ * names each row's sequence (NULL: row b is sequence b); calls that change
+ * sequences take each once, gather and attention may read one in several rows.
  * ---------------------------------------------------------------------- */
 typedef struct {
   uint8_t* k_codes;
