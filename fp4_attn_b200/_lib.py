@@ -89,11 +89,14 @@ def load() -> ctypes.CDLL:
 
 def call(name: str, *args) -> None:
     """Call an entry point; a non-zero status raises RuntimeError with the library's message."""
-    L = load()
-    rc = getattr(L, name)(*args)
+    rc = getattr(load(), name)(*args)
     if rc != 0:
-        msg = L.fp4attn_last_error().decode(errors="replace")
-        raise RuntimeError(f"{name} failed ({rc}): {msg}")
+        _fail(name, rc)
+
+
+def _fail(name: str, rc: int) -> None:
+    msg = load().fp4attn_last_error().decode(errors="replace")
+    raise RuntimeError(f"{name} failed ({rc}): {msg}")
 
 
 def launch_count() -> int:
@@ -106,9 +109,16 @@ def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
-def raw_stream(device_index: int) -> int:
-    """The same by device index, without making a Stream object (2 us of a small call)."""
-    return torch._C._cuda_getCurrentRawStream(device_index)
+def call_on(device_index: int, name: str, *args) -> None:
+    """call() with device device_index current, as launches and kernel attributes need it, and that device's current
+    stream as the last argument."""
+    if torch._C._cuda_getDevice() != device_index:
+        with torch.cuda.device(device_index):
+            return call_on(device_index, name, *args)
+    # (without making a Stream object, which takes 2 us)
+    rc = getattr(load(), name)(*args, torch._C._cuda_getCurrentRawStream(device_index))
+    if rc != 0:
+        _fail(name, rc)
 
 
 def require_cuda(*tensors: torch.Tensor) -> None:

@@ -105,12 +105,14 @@ class PagedNVFP4Cache:
 
     # ------------------------------------------------------------ helpers
     def _call(self, name: str, *args) -> None:
-        _lib.call(name, self._ref, *args, _lib.raw_stream(self._index))
+        _lib.call_on(self._index, name, self._ref, *args)
 
     def _workspace(self, B: int, Hq: int, N: int) -> torch.Tensor:
         need = self._work_bytes.get((B, Hq, N))
         if need is None:
-            need = self._work_bytes[B, Hq, N] = _lib.load().fp4paged_attention_workspace_size(B, Hq, self.num_kv_heads, N)
+            with torch.cuda.device(self._index):  # the size goes by the device's SMs
+                need = _lib.load().fp4paged_attention_workspace_size(B, Hq, self.num_kv_heads, N)
+            self._work_bytes[B, Hq, N] = need
         if not self._spaces or self._spaces[-1].numel() < need:
             grown = max(need, 2 * self._spaces[-1].numel()) if self._spaces else need
             self._spaces.append(torch.empty(grown, dtype=torch.uint8, device=self.device))
@@ -270,6 +272,8 @@ def tree_attention(q: torch.Tensor, cache: PagedNVFP4Cache, mask: torch.Tensor |
         return out
     if workspace is None:
         workspace = cache._workspace(B, Hq, N)
+    elif workspace.device != device or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous buffer on {device}")
     cache._call("fp4paged_attention", q.data_ptr(), in_code, B, Hq, N, sB, sH, sN, mp, mB, mI, mJ,
                 None if counts is None else _int32("counts", counts, (B,), device), cache._rows(seqs, B),
                 D ** -0.5 if scaling is None else float(scaling), out.data_ptr(), out_code, workspace.data_ptr(),

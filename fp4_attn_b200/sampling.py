@@ -74,8 +74,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     p = _per_row("top_p", top_p, R, torch.float32, dev, 1.0)
     m = _per_row("min_p", min_p, R, torch.float32, dev, 0.0)
     ptr = _lib.ptr
-    _lib.call("fp4_sample", x.data_ptr(), code, R, V, ld, u.data_ptr(), ptr(t), ptr(k), ptr(p), ptr(m),
-              tokens.data_ptr(), logprobs.data_ptr(), _lib.raw_stream(dev.index))
+    _lib.call_on(dev.index, "fp4_sample", x.data_ptr(), code, R, V, ld, u.data_ptr(), ptr(t), ptr(k), ptr(p),
+                 ptr(m), tokens.data_ptr(), logprobs.data_ptr())
     return tokens, logprobs
 
 
@@ -107,6 +107,6 @@ def accept_tree(parents: torch.Tensor, tokens: torch.Tensor, sampled: torch.Tens
     nxt = torch.empty(B, dtype=torch.int64, device=dev)
     parents, tokens, sampled = parents.contiguous(), tokens.contiguous(), sampled.contiguous()
     counts = None if counts is None else counts.contiguous()
-    _lib.call("fp4_accept_tree", parents.data_ptr(), tokens.data_ptr(), sampled.data_ptr(), _lib.ptr(counts), B, N,
-              keep.data_ptr(), n.data_ptr(), nxt.data_ptr(), _lib.stream_of(parents))
+    _lib.call_on(dev.index, "fp4_accept_tree", parents.data_ptr(), tokens.data_ptr(), sampled.data_ptr(),
+                 _lib.ptr(counts), B, N, keep.data_ptr(), n.data_ptr(), nxt.data_ptr())
     return keep, n, nxt

@@ -119,3 +119,15 @@ def test_zero_values_among_small_ones(exponent, dtype, largest, N, G):
     tol = U[dtype] * ref.abs() + e * share + 2.0 ** -36 * top + 2.0 ** -24 * (dtype == torch.float16)
     err = (o[0].double() - ref).abs()
     assert (err <= tol).all(), float((err / tol).max())
+
+
+def test_a_workspace_elsewhere_is_refused():
+    from fp4_attn_b200.paged_cache import tree_attention
+    cache = cache_of(*(torch.randn(1, 2, 9, D, device=DEV) for _ in range(2)))
+    q = torch.randn(1, 4, 2, D, device=DEV)
+    size = 1 << 22
+    for w in (torch.empty(size, dtype=torch.uint8), torch.empty(size, 2, dtype=torch.uint8, device=DEV)[:, 0]):
+        with pytest.raises(ValueError, match="workspace"):
+            tree_attention(q, cache, workspace=w)
+    good = torch.empty(size, dtype=torch.uint8, device=DEV)
+    assert torch.equal(tree_attention(q, cache, workspace=good), tree_attention(q, cache))
