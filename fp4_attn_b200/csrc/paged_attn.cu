@@ -1098,20 +1098,21 @@ struct Layout {
 
 int64_t piece(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
-Layout layout_of(int B, int Hq, int Hkv, int N, bool fp32) {
+// SMs of the current device (148 where there is none to ask).
+int sm_count() {
+  int dev = 0, n = 0;
+  return cudaGetDevice(&dev) == cudaSuccess &&
+                 cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0
+             ? n
+             : 148;
+}
+
+Layout layout_of(int B, int Hq, int Hkv, int N, bool fp32, int sms) {
   Layout L;
   const int64_t rows = (int64_t)N * (Hq / Hkv), tok = (int64_t)B * N;
   L.NB = rows_per_tile(rows, fp32);
   L.RT = (int)((rows + L.NB - 1) / L.NB);
   L.nw = (N + 31) / 32;
-  static int sms = 0;
-  if (!sms) {
-    int dev = 0, n = 0;
-    sms = cudaGetDevice(&dev) == cudaSuccess &&
-                  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0
-              ? n
-              : 148;
-  }
   L.grid = sms;
   const int64_t qrows = (int64_t)B * Hkv * L.RT * L.NB;
   L.scales = piece(qrows * PG_ROW);
@@ -1122,6 +1123,10 @@ Layout layout_of(int B, int Hq, int Hkv, int N, bool fp32) {
   L.part = L.first + piece((int64_t)(B + 1) * 4);
   L.bytes = L.part + piece((int64_t)L.grid * 2 * L.NB * (PG_D + 2) * 4);
   return L;
+}
+
+int64_t bytes_of(int B, int Hq, int Hkv, int N, int sms) {
+  return std::max(layout_of(B, Hq, Hkv, N, false, sms).bytes, layout_of(B, Hq, Hkv, N, true, sms).bytes);
 }
 
 template <typename... KArgs, typename... Args>
@@ -1174,7 +1179,7 @@ using namespace fp4;
 
 extern "C" int64_t fp4paged_attention_workspace_size(int B, int Hq, int Hkv, int N) {
   if (B <= 0 || N <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv) return -1;
-  return std::max(layout_of(B, Hq, Hkv, N, false).bytes, layout_of(B, Hq, Hkv, N, true).bytes);
+  return bytes_of(B, Hq, Hkv, N, sm_count());
 }
 
 extern "C" int fp4paged_attention(const fp4paged_cache* cache, const void* q, int in_dtype, int B, int Hq, int N,
@@ -1190,11 +1195,12 @@ extern "C" int fp4paged_attention(const fp4paged_cache* cache, const void* q, in
   if (B == 0 || N == 0) return FP4ATTN_OK;
   if (!q || !out || !workspace) return set_error(FP4ATTN_ERR_ARG, "null pointer");
   if (in_dtype < 0 || in_dtype > 2 || out_dtype < 0 || out_dtype > 2) return set_error(FP4ATTN_ERR_ARG, "bad dtype");
-  const int64_t need = fp4paged_attention_workspace_size(B, Hq, H, N);
+  const int sms = sm_count();
+  const int64_t need = bytes_of(B, Hq, H, N, sms);
   if ((uintptr_t)workspace % 256 || workspace_bytes < need)
     return set_error(FP4ATTN_ERR_ARG, "workspace of %lld bytes, %lld needed (256-byte aligned)",
                      (long long)workspace_bytes, (long long)need);
-  const Layout L = layout_of(B, Hq, H, N, out_dtype == FP4_DT_F32);
+  const Layout L = layout_of(B, Hq, H, N, out_dtype == FP4_DT_F32, sms);
   // grid limits, 32-bit rows, and the tensor maps' 32-bit row coordinate
   if (B > 65535 || (int64_t)H * L.RT > 65535 || (int64_t)N * (Hq / H) > INT32_MAX / 2 ||
       (int64_t)B * N > INT32_MAX / 2)
