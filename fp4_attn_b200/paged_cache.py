@@ -202,12 +202,12 @@ class PagedNVFP4Cache:
 
 
 def tree_mask(parents: torch.Tensor) -> torch.Tensor:
-    """Mask of drafted trees for ``tree_attention``: parents [B, N] (a node's parent comes before it, -1: none)
-    -> bool [B, N, N], node i sees itself and its ancestors."""
+    """Mask of drafted trees for ``tree_attention``: parents [B, N] (a node's parent comes before it, -1: none;
+    what is not before it counts as none) -> bool [B, N, N], node i sees itself and its ancestors."""
     N = parents.shape[-1]
     nodes = torch.arange(N, device=parents.device)
     at, seen = nodes.expand(parents.shape), None
-    parents = parents.long()
+    parents = torch.where(parents < nodes, parents, -1).long()
     for _ in range(N):
         hit = at[..., None] == nodes
         seen = hit if seen is None else seen | hit
