@@ -113,9 +113,9 @@ __device__ __forceinline__ int row_of(const int32_t* off, int B, int i) {
 // Whether another row of the call names row b's sequence s: two rows would change one sequence at the same time.  The
 // block looks through all rows; every thread of it takes part.
 __device__ __forceinline__ bool named_twice(const int32_t* seqs, int B, int b, int s) {
+  if (!seqs) return false;
   bool twice = false;
-  if (seqs)
-    for (int j = threadIdx.x; j < B; j += blockDim.x) twice |= j != b && seqs[j] == s;
+  for (int j = threadIdx.x; j < B; j += blockDim.x) twice |= j != b && seqs[j] == s;
   return __syncthreads_or(twice);
 }
 
@@ -252,10 +252,11 @@ __device__ __forceinline__ void drop_pages(const fp4paged_cache& c, int s, int o
 __global__ void __launch_bounds__(128) truncate_kernel(fp4paged_cache c, const int32_t* lens, const int32_t* seqs) {
   const int s = pg_seq(c, seqs, blockIdx.x);
   const int old = s < 0 ? 0 : c.lens[s], len = lens ? max(0, min(lens[blockIdx.x], old)) : 0;
-  if (named_twice(seqs, gridDim.x, blockIdx.x, s) || s < 0) {  // (every thread has read lens[s])
+  if (named_twice(seqs, gridDim.x, blockIdx.x, s) || s < 0) {
     if (threadIdx.x == 0) atomicOr(c.status, PG_BAD_SEQ);
     return;
   }
+  __syncthreads();  // every thread has read lens[s]
   drop_pages(c, s, old, len);
 }
 
