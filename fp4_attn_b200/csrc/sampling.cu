@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
   const float t0 = a.temperature ? a.temperature[r] : 1.0f, temp = t0 > 0.0f ? fmaxf(t0, 1e-30f) : 1.0f;
   const int k = a.top_k ? a.top_k[r] : 0;
   const float top_p = a.top_p ? a.top_p[r] : 1.0f, min_p = a.min_p ? a.min_p[r] : 0.0f;
-  const bool greedy = !(t0 > 0.0f) || !(min_p <= 1.0f);  // (min_p above 1: nothing is left but the first)
+  const bool greedy = !(t0 > 0.0f);
   const bool by_k = !greedy && k > 0 && k < a.V, by_p = !greedy && top_p < 1.0f;
   // w = 2^((x - max) log2(e) / T): the factor in two parts, so that the product is rounded once
   const double f = 1.4426950408889634 / (double)temp;
@@ -719,7 +719,10 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
   }
 
   // ----------------------------------------------------------------- the draw
-  const u64 least = (u64)ceil((double)fmaxf(min_p, 0.0f) * (double)SP_ONE);
+  // min_p above 1 leaves the first of the largest: they are what is kept, and the draw takes its lowest
+  const bool only_first = !(min_p <= 1.0f);
+  if (only_first) cut = {sp_key(mx), INT32_MAX};
+  const u64 least = (u64)ceil((double)fmaxf(fminf(min_p, 1.0f), 0.0f) * (double)SP_ONE);
   // (key 0 is below every logit's)
   const float edge = cut.key == 0u ? -INFINITY : logit_of(cut.key);
   auto kept = [&](float v, int index) -> u64 {
@@ -740,7 +743,7 @@ __global__ void __launch_bounds__(STREAM ? SP_STREAM_THREADS : SP_HELD_THREADS, 
     each_near(mx - edge <= near_reach, [&](float v) { return v >= edge; }, [&](float v, int index) { own += kept(v, index); });
   }
   const Before s = row_scan(own);  // its barrier is behind the last access to another CTA's memory
-  const u64 target = min((u64)floor((double)a.u[r] * (double)s.total), s.total - 1);
+  const u64 target = only_first ? 0 : min((u64)floor((double)a.u[r] * (double)s.total), s.total - 1);
   row_find(s, target, kept, [&](float v, int index) {
     a.tokens[r] = index;
     if (a.logprobs) a.logprobs[r] = (v - mx) / temp - logz;
