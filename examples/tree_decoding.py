@@ -10,9 +10,11 @@ same random numbers (one per position):
   and ``compact`` keeps the accepted tokens and frees the pages of the rest.
 
 Nothing in a step waits for the host.  A token's K, V and query are quantized by
-themselves and P is not quantized, so what else was drafted does not change a
-token's output: both ways generate the same tokens.  The beam at the end forks
-a sequence (its full pages are shared) and frees it.
+themselves and P is not quantized, so what else was drafted changes a token's
+output in its last places only (the order of sums and the maximum that weights
+are rounded under are those of the call): both ways generate the same tokens
+unless a random number lies that near a boundary between two.  The beam at the
+end forks a sequence (its full pages are shared) and frees it.
 
     python examples/tree_decoding.py [--steps 48] [--nodes 9]
 """

@@ -274,7 +274,13 @@ struct Share {
 // 16 rows and 32 keys only 90, hence tiles of 256 keys and as many rows per warp as its registers hold.
 // With 64 rows it is about 10300 warp instructions a tile, 2500 of them V's widening and 1400 the exponentials.
 // Measured, all three kernels: 8 x 32768 keys, 8 heads, 8 rows: 99 us, 3.1 TB/s of 304 MB (46 us at a plain copy's
-// rate); 2 x 65536 keys, 8 heads, 512 rows: 554 us, 250 TFLOP/s in O^T (83 us at the fp16 rate of a large product).
+// rate); 2 x 65536 keys, 8 heads, 512 rows: 568 us, 242 TFLOP/s in O^T (83 us at the fp16 rate of a large product).
+//
+// Roundings to fewer than 32 bits.  fp32 outputs (PL 2): W is two fp16 planes, 2^-22 of it together, and each tile's
+// product is added up in registers.  16-bit outputs (PL 1): W is one plane, off by up to 2^-11 of itself, as an fp16
+// output is of its own and a quarter of what a bf16 one is, and the keys' errors average out (drafted trees in fp16,
+// relative error against 64 bits: 2.3e-4, with W in 32 bits 2.1e-4; in bf16 the same); O adds up in the tensor cores,
+// which cut off, 2e-6 of it after 14 tiles of 128 keys.  A second plane would double the O^T products.
 constexpr uint32_t KC = TK * PG_ROW, KS = TK * PG_SF, KG = TK * 4;
 constexpr uint32_t O_VC = KC, O_KS = 2 * KC, O_VS = O_KS + KS, O_KG = O_VS + KS, O_VG = O_KG + KG;
 constexpr uint32_t STAGE = O_VG + KG;  // K codes, V codes, K scales, V scales, K g, V g: 38 KB

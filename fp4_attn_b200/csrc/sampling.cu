@@ -16,7 +16,7 @@
 // keeps the logits near the maximum, which are what the rest needs, in shared memory.
 //
 // One row of 32000: 16 us, a chain of about a dozen exchanges and barriers.  512 rows of 131072 fp32 under
-// top_p: 183 us, 1.5 TB/s (41 us at a plain copy's rate).  There the first pass (maximum) runs at the
+// top_p: 180 us, 1.5 TB/s (41 us at a plain copy's rate).  There the first pass (maximum) runs at the
 // memory's rate and is a fifth of a row's time; the second (weights, sum, histogram), half of it, is bound
 // by instructions (about 16 per logit, half of them for the weight); what follows by latencies.
 #include <cooperative_groups.h>

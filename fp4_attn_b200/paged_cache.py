@@ -230,7 +230,9 @@ def tree_attention(q: torch.Tensor, cache: PagedNVFP4Cache, mask: torch.Tensor |
     q is quantized to NVFP4 as the cache's tokens are (per token over its Hq*D
     channels), QK^T runs on the FP4 tensor cores, softmax in fp32, and P is not
     quantized: blocks of P would run over sibling nodes, so that a token's
-    output would depend on what else was drafted.  The output has q's dtype
+    output would depend on what else was drafted.  (As it is, only its last
+    places do: how the keys are shared out, and the maximum that weights are
+    rounded under, go by all rows of the call.)  The output has q's dtype
     unless out or out_dtype says otherwise.  V tokens whose largest value is
     below 2^-100 count as 0.
 
