@@ -781,7 +781,8 @@ __global__ void __launch_bounds__(Cfg<NB, PL>::THREADS, 1)
         // y = x - m + W_BIAS, x = S scaling log2(e) + log2(g_v); -inf marks what a row does not see.  x is rounded by
         // itself, as where m is made of it, and W_BIAS - m is rounded down: once m has moved, y <= W_BIAS holds to the
         // bit for x of all sizes, and the key that has the maximum keeps a weight of 1 or more.  (Rounded as one sum, y
-        // is off by up to x's last place, which passes W_SLACK from 2^27 on; 2 x 65536 keys, 512 rows: 554 us so, now 566.)
+        // is off by up to x's last place, which passes W_SLACK from 2^27 on; 2 x 65536 keys, 512 rows: 554 us so, 566
+        // like this.)
         float y[2][16];
 #pragma unroll 1
         for (bool moved = false;; moved = true) {  // twice at most

@@ -30,10 +30,10 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     In order of (logit descending, index ascending) a row keeps its first
     top_k tokens (<= 0: all), of those the shortest prefix with at least a share
     top_p of their probability (>= 1: all), of those the ones at least min_p
-    times as probable as the first (above 1: that one only).  The token is where the running sum of the
-    kept probabilities, in index order, passes u.  temperature <= 0 takes the
-    largest logit (the lowest index among equals).  Each parameter is a number
-    or a tensor of a value per row.
+    times as probable as the first (above 1: that one only).  The token is
+    where the running sum of the kept probabilities, in index order, passes u.
+    temperature <= 0 takes the largest logit (the lowest index among equals).
+    Each parameter is a number or a tensor of a value per row.
 
     logprobs: log softmax(logits / temperature) of the token, before the
     filters (temperature 1 for a greedy row).  NaN logits count as -inf, +inf as

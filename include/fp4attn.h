@@ -419,9 +419,10 @@ int fp4paged_attention(const fp4paged_cache* cache, const void* q, int in_dtype,
  * ascending) a row keeps the first top_k[r] (<= 0: all), of those the
  * shortest prefix with a share of at least top_p[r] (>= 1: all), of those
  * the ones with a weight of at least min_p[r] of the largest; always the
- * first (above 1: only that).  The token is the first kept index i (in index order) whose running
- * sum exceeds floor(u * sum).  temperature <= 0: the lowest index of the
- * largest logit.  NaN counts as -inf, +inf as the largest finite value.
+ * first (min_p above 1: only that one).  The token is the first kept index i
+ * (in index order) whose running sum exceeds floor(u * sum).  temperature
+ * <= 0: the lowest index of the largest logit.  NaN counts as -inf, +inf as
+ * the largest finite value.
  * logprob[r] (may be NULL) = log softmax(x / temperature)[token], before the
  * filters (temperature 1 for a greedy row).  A row without a finite logit:
  * token -1, logprob -inf.  NULL temperature / top_k / top_p / min_p: 1 / 0 / 1 /
